@@ -212,7 +212,8 @@ def run(s: dict):
             dw[i] = s["dy"][a:b].float().t() @ s["x"][a:b].float()
         return dx.to(s["x"].dtype), dw.to(DTYPES[case["out"]])
     if op == "linear8":
-        xs = s["x"].float().abs().amax(1) / 127.0
+        # torch multiplies by the rounded 1 / 127 in 32 bits, which is not the rounded quotient
+        xs = (s["x"].abs().amax(1).double() / 127.0).float()
         # a quotient next to a half needs more than 32 bits to round to the right side of it
         xq = (s["x"].double() / xs.double()[:, None]).round().clamp(-127, 127)
         xq = torch.where(xs[:, None] > 0, xq, torch.zeros_like(xq))
@@ -257,7 +258,7 @@ def exact(case: dict, seed: int):
     if case["op"] == "linear8":
         # a row's scale is its largest magnitude over 127, held in 32 bits; ties round to the even integer
         peak = torch.maximum(s["x"].max(1).values, -s["x"].min(1).values)
-        scale = (peak.to(torch.float32) / 127.0).to(f64)
+        scale = (peak.to(f64) / 127.0).to(torch.float32).to(f64)
         q = torch.round(s["x"].to(f64) / torch.where(scale > 0, scale, torch.ones_like(scale))[:, None])
         q = q.clamp_(-127, 127)
     else:
