@@ -1,8 +1,8 @@
 """Build recipe for the in-tree native library ``lib/libemmy_b200.so``.
 
 The launcher is plain C++ over the CUDA driver API (libcuda and libnccl are
-opened at run time); the one precompiled kernel of the library
-(csrc/emmy_noalloc.cu) is built with nvcc for sm_100a and uses a private,
+opened at run time); the precompiled kernels of the library
+(csrc/*.cu) are built with nvcc for sm_100a and use a private,
 statically linked CUDA runtime.  The library builds and loads on machines
 without a GPU.
 """
@@ -18,9 +18,10 @@ REPO = PKG.parent
 LIB_DIR = PKG / "lib"
 RUNTIME_SO = LIB_DIR / "libemmy_b200.so"
 SOURCES = [PKG / "csrc" / "emmy_runtime.cpp"]
-CUDA_SOURCES = [PKG / "csrc" / "emmy_noalloc.cu", PKG / "csrc" / "emmy_xchg.cu"]
+CUDA_SOURCES = [PKG / "csrc" / "emmy_noalloc.cu", PKG / "csrc" / "emmy_xchg.cu",
+                PKG / "csrc" / "emmy_products.cu"]
 HEADERS = [REPO / "include" / "emmy_b200.h", REPO / "include" / "emmy_launch_record.h",
-           PKG / "csrc" / "emmy_xchg_dev.cuh"]
+           PKG / "csrc" / "emmy_xchg_dev.cuh", PKG / "csrc" / "emmy_sm100.cuh"]
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 CUDA_INC = CUDA_HOME / "include"
 CUDA_LIB = CUDA_HOME / "lib64"

@@ -199,6 +199,60 @@ int emmy_graph_destroy(emmy_graph_t g);
 #define EMMY_NOALLOC_MAX_ELEMENTS (1ull << 36)
 int emmy_sum_f32_noalloc(int dev, const float *x, uint64_t n, float *out, uint64_t stream);
 
+/* Matrix products that a static KernelOp cannot express (no counterpart in the
+ * reference): products grouped by expert with sizes known only on the device,
+ * their gradients, and products of 8-bit integers.  All are asynchronous on
+ * `stream`, allocate nothing, keep no state between calls and never
+ * synchronise, so they can be recorded into graphs and overlap each other.
+ * Extents and strides are counted in elements; an innermost stride not given
+ * is 1.  Outputs must not overlap inputs.  Extents of 0 are fine.
+ *
+ * Groups: `offsets` (device, experts + 1 words) names expert e's rows
+ * [offsets[e], offsets[e + 1]).  Rows outside every group are neither used
+ * nor written.  An offset below an earlier one counts as that earlier one and
+ * one beyond `rows` as `rows`, so no value leads outside the buffers.
+ *
+ * Types: EMMY_BF16 or EMMY_F16 operands with f32 accumulation, outputs of the
+ * operands' type or EMMY_F32; EMMY_S8 operands accumulate in s32, which is
+ * exact for k <= EMMY_PRODUCTS_MAX_K8.
+ *
+ *   emmy_grouped_matmul     out[r, :] = sum_k x[r, k] * w[e, :, k] for the rows r
+ *                           of expert e.  One of w's strides over n and k is 1.
+ *                           The rows' gradient is the same call on dy with the
+ *                           two strides (and n and k) exchanged.
+ *   emmy_grouped_matmul_dw  dw[e, n, :] = sum over expert e's rows of
+ *                           dy[r, n] * x[r, :]; zeros for an expert without rows.
+ *   emmy_int8_matmul        out[r, n] = (sum_k xq[r, k] * wq[e, n, k]) * x_scale[r]
+ *                           * w_scale[e, n] (+ bias[e, n]); w_scale and bias are
+ *                           dense [experts, n], bias may be NULL, and offsets NULL
+ *                           means one group of all rows (experts must be 1).
+ *   emmy_quantize_rows      scale[r] = max |x[r, :]| / 127 rounded to f32, q[r, c] =
+ *                           x[r, c] / scale[r] rounded to the nearest integer (exact
+ *                           ties to even), within [-127, 127].  A row of zeros
+ *                           gives scale 0 and zeros; a row that holds an
+ *                           infinity or NaN gives scale NaN and zeros.
+ *   emmy_products_status    reads and clears the device's EMMY_STATUS_* bits of
+ *                           these kernels (a bounded wait that ran out, whose
+ *                           outputs are then undefined); synchronises the device. */
+#define EMMY_F32 0
+#define EMMY_BF16 1
+#define EMMY_F16 2
+#define EMMY_PRODUCTS_MAX_EXPERTS 1024
+#define EMMY_PRODUCTS_MAX_K8 131071
+int emmy_grouped_matmul(int dev, int dtype, int out_dtype, const void *x, int64_t x_stride, const void *w,
+                        int64_t w_stride_e, int64_t w_stride_n, int64_t w_stride_k, const int32_t *offsets, void *out,
+                        int64_t out_stride, int64_t rows, int64_t experts, int64_t n, int64_t k, uint64_t stream);
+int emmy_grouped_matmul_dw(int dev, int dtype, int out_dtype, const void *dy, int64_t dy_stride, const void *x,
+                           int64_t x_stride, const int32_t *offsets, void *dw, int64_t dw_stride_e,
+                           int64_t dw_stride_n, int64_t rows, int64_t experts, int64_t n, int64_t k, uint64_t stream);
+int emmy_int8_matmul(int dev, int out_dtype, const int8_t *xq, int64_t x_stride, const float *x_scale,
+                     const int8_t *wq, int64_t w_stride_e, int64_t w_stride_n, const float *w_scale,
+                     const float *bias, const int32_t *offsets, void *out, int64_t out_stride, int64_t rows,
+                     int64_t experts, int64_t n, int64_t k, uint64_t stream);
+int emmy_quantize_rows(int dev, int dtype, const void *x, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
+                       int64_t rows, int64_t k, uint64_t stream);
+int emmy_products_status(int dev, uint32_t *status);
+
 /* The C4 step on N GPUs as ONE kernel per GPU (no counterpart in the
  * reference, which has no multi-GPU path): the full-array sum of this GPU's
  * shard fused with the cross-GPU combine over NVLink peer memory.
