@@ -15,11 +15,11 @@
 // The group boundaries are read on the device; a launch covers any of them, so no call waits for
 // the host and a recorded graph follows new boundaries.
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -28,177 +28,14 @@
 
 extern "C" int emmy_record_error(int code, const char *msg);  // emmy_runtime.cpp (not exported)
 
-// Status bits of this file's kernels, one word for each device (the name is private to this file).
-#define emmy_status g_products_status
-extern "C" {
-static __device__ unsigned int g_products_status = 0u;
-}
+// Status bits of this file's kernels, one word for each device; private to this file.
+static __device__ unsigned int emmy_status = 0u;
+#define EMMY_STATUS_DEFINED
+
+#include "emmy_products_dev.cuh"
+#include "emmy_products_tc.cuh"
 
 namespace {
-
-constexpr int kMaxExperts = EMMY_PRODUCTS_MAX_EXPERTS;
-constexpr int kS8 = 3;  // operand code of 8-bit products beside EMMY_F32, EMMY_BF16 and EMMY_F16
-
-// One product, as the kernels see it.  Strides are in elements.
-struct Product {
-    const void *a;  // A(m, k) of expert e at a[e * a_e + m * a_m + k * a_k]  (dw: k counts from the group's start)
-    const void *b;  // B(c, k): forward b[(begin_e + c) * b_c + k], dw b[(begin_e + k) * b_k + c]
-    void *out;      // forward out[(begin_e + c) * out_c + m], dw out[e * out_e + c * out_c + m]
-    const int32_t *offsets;
-    const float *x_scale;  // [rows], or NULL: plain sums
-    const float *w_scale;  // [experts, m]
-    const float *bias;     // [experts, m], or NULL
-    int64_t a_e, a_m, a_k, b_c, b_k, out_e, out_c;
-    int64_t m, c, k;  // extents; c counts only for dw, k only for the forward form
-    int64_t rows;
-    int experts;
-    int out_type;
-    bool dw;
-};
-
-// ---------------------------------------------------------------- groups
-
-// Boundaries of the groups in shared memory: row[e] .. row[e + 1] are expert e's rows, after every
-// offset was brought into [0, rows] and up to the largest before it; tiles[e] counts the column
-// tiles of the experts before e.
-struct Groups {
-    int row[kMaxExperts + 1];
-    int tiles[kMaxExperts + 1];
-};
-
-// Filled by one whole warp: each lane takes a run of consecutive experts; running maxima and sums
-// cross the lanes in two warp scans.
-__device__ __forceinline__ void load_groups(Groups &g, const Product &p, int col_tile) {
-    const int lane = threadIdx.x & 31, e = p.experts, rows = static_cast<int>(p.rows);
-    if (!p.offsets) {
-        if (lane == 0) {
-            g.row[0] = 0;
-            g.row[1] = rows;
-        }
-    } else {
-        const int per = (e + 1 + 31) / 32, i0 = lane * per, i1 = min(e + 1, i0 + per);
-        int top = 0;
-        for (int i = i0; i < i1; ++i) {
-            top = max(top, min(max(p.offsets[i], 0), rows));
-            g.row[i] = top;
-        }
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, top, d);
-            if (lane >= d) top = max(top, up);
-        }
-        const int before = __shfl_up_sync(0xffffffffu, top, 1);
-        if (lane > 0)
-            for (int i = i0; i < i1; ++i) g.row[i] = max(g.row[i], before);
-    }
-    __syncwarp();
-    const int per = (e + 31) / 32, i0 = min(e, lane * per), i1 = min(e, i0 + per);
-    auto tiles_of = [&](int i) {
-        return p.dw ? static_cast<int>((p.c + col_tile - 1) / col_tile)
-                    : (g.row[i + 1] - g.row[i] + col_tile - 1) / col_tile;
-    };
-    int sum = 0;
-    for (int i = i0; i < i1; ++i) sum += tiles_of(i);
-    int upto = sum;
-    for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += up;
-    }
-    int at = upto - sum;
-    for (int i = i0; i < i1; ++i) {
-        g.tiles[i] = at;
-        at += tiles_of(i);
-    }
-    if (lane == 31) g.tiles[e] = upto;
-    __syncwarp();
-}
-
-__device__ __forceinline__ void store_out(void *out, int type, int64_t i, float v) {
-    if (type == EMMY_BF16) {
-        static_cast<__nv_bfloat16 *>(out)[i] = __float2bfloat16_rn(v);
-    } else if (type == EMMY_F16) {
-        static_cast<__half *>(out)[i] = __float2half_rn(v);
-    } else {
-        static_cast<float *>(out)[i] = v;
-    }
-}
-
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(float v) { return v; }
-
-template <typename Acc, typename T>
-__device__ __forceinline__ Acc load_as(T v) {
-    if constexpr (sizeof(T) == 1) return v;
-    else return to_float(v);
-}
-
-// ---------------------------------------------------------------- products on CUDA cores
-
-// 64 x 64 tiles on 256 threads, 16 of k at a time through shared memory: any stride, alignment and
-// extent.  Sums are held in f32 (s32 for 8-bit operands).
-template <typename T, typename Acc>
-__global__ void __launch_bounds__(256) product_simt_kernel(const Product p) {
-    constexpr int TM = 64, TC = 64, TK = 16;
-    __shared__ Groups g;
-    __shared__ Acc sa[TK][TM + 1];
-    __shared__ Acc sb[TK][TC + 1];
-    if (threadIdx.x < 32) load_groups(g, p, TC);
-    __syncthreads();
-    const int64_t mt = (p.m + TM - 1) / TM, total = mt * g.tiles[p.experts];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const T *a = static_cast<const T *>(p.a), *b = static_cast<const T *>(p.b);
-    int e = 0;
-    for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-        while (t >= mt * g.tiles[e + 1]) ++e;
-        const int64_t r = t - mt * g.tiles[e];
-        const int64_t m0 = r % mt * TM, c0 = r / mt * TC;
-        const int64_t begin = g.row[e], count = g.row[e + 1] - g.row[e];
-        const int64_t cend = p.dw ? p.c : count, kend = p.dw ? count : p.k;
-        const T *ae = a + (p.dw ? begin * p.a_k : e * p.a_e);
-        const T *be = b + begin * (p.dw ? p.b_k : p.b_c);
-        Acc acc[4][4] = {};
-        for (int64_t k0 = 0; k0 < kend; k0 += TK) {
-            for (int i = threadIdx.x; i < TK * TM; i += 256) {
-                // neighbouring threads follow the axis that is contiguous in memory
-                const int mm = p.a_k == 1 ? i / TK : i % TM, kk = p.a_k == 1 ? i % TK : i / TM;
-                const int64_t gm = m0 + mm, gk = k0 + kk;
-                sa[kk][mm] = gm < p.m && gk < kend ? load_as<Acc>(ae[gm * p.a_m + gk * p.a_k]) : Acc(0);
-            }
-            for (int i = threadIdx.x; i < TK * TC; i += 256) {
-                const int cc = p.b_k == 1 ? i / TK : i % TC, kk = p.b_k == 1 ? i % TK : i / TC;
-                const int64_t gc = c0 + cc, gk = k0 + kk;
-                sb[kk][cc] = gc < cend && gk < kend ? load_as<Acc>(be[gc * p.b_c + gk * p.b_k]) : Acc(0);
-            }
-            __syncthreads();
-            for (int kk = 0; kk < TK; ++kk) {
-                Acc av[4], bv[4];
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) av[i] = sa[kk][tx + 16 * i];
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) bv[i] = sb[kk][ty + 16 * i];
-                #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] += av[i] * bv[j];
-            }
-            __syncthreads();
-        }
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t m = m0 + tx + 16 * i, c = c0 + ty + 16 * j;
-                if (m >= p.m || c >= cend) continue;
-                float v = static_cast<float>(acc[i][j]);
-                if (p.x_scale) {
-                    v = v * p.x_scale[begin + c] * p.w_scale[e * p.m + m];
-                    if (p.bias) v += p.bias[e * p.m + m];
-                }
-                store_out(p.out, p.out_type, (p.dw ? e * p.out_e : begin * p.out_c) + c * p.out_c + m, v);
-            }
-        }
-    }
-}
 
 // ---------------------------------------------------------------- row quantization
 
@@ -288,22 +125,152 @@ constexpr int64_t kMaxExtent = (1ll << 31) - 1;
 
 bool bad_extent(int64_t v) { return v < 0 || v > kMaxExtent; }
 
-int launch_product(const char *name, int dev, int operands, const Product &p, uint64_t stream) {
+// ---- tensor maps
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+    static const EncodeTiledFn fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    return fn;
+}
+
+// An operand as TMA sees it: `inner` contiguous values, then one or two strided extents (elements).
+struct Operand {
+    const void *base;
+    int64_t inner, rows, row_stride, mats, mat_stride;
+};
+
+// TMA takes 16-byte aligned bases and strides; where an extent is 1 its stride is free, so any
+// valid one stands in for it.
+bool tma_ready(Operand &o, int esize) {
+    if (o.inner < 1 || o.rows < 1 || o.mats < 1) return false;
+    const int64_t unit = 16 / esize;
+    if (o.rows == 1) o.row_stride = (o.inner + unit - 1) / unit * unit;
+    if (o.mats == 1) o.mat_stride = (o.rows * o.row_stride + unit - 1) / unit * unit;
+    return reinterpret_cast<uintptr_t>(o.base) % 16 == 0 && o.row_stride % unit == 0 && o.mat_stride % unit == 0 &&
+           o.row_stride >= o.inner && o.mat_stride > 0 && o.row_stride * esize < (1ll << 40) &&
+           o.mat_stride * esize < (1ll << 40);
+}
+
+bool encode(CUtensorMap *map, const Operand &o, CUtensorMapDataType type, int esize, int rank, uint32_t box_inner,
+            uint32_t box_rows) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.inner), static_cast<cuuint64_t>(o.rows),
+                                static_cast<cuuint64_t>(o.mats)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.row_stride) * esize,
+                                   static_cast<cuuint64_t>(o.mat_stride) * esize};
+    const cuuint32_t box[3] = {box_inner, box_rows, 1}, step[3] = {1, 1, 1};
+    return encode_tiled()(map, type, rank, const_cast<void *>(o.base), dims, strides, box, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ---- launches
+
+constexpr int kSms = 148;
+
+struct Call {
+    const char *name;
+    int dev;
+    cudaStream_t stream;
+};
+
+int launched(const Call &call, cudaError_t err) {
+    if (err == cudaSuccess) return EMMY_OK;
+    cudaGetLastError();  // the launch's own error does not stay behind for the caller's next check
+    return report(EMMY_ERR_CUDA, "%s: launch: %s", call.name, cudaGetErrorString(err));
+}
+
+template <bool I8, int BN, bool TMA>
+int launch_tc(const Call &call, const Product &p, const Layout &lay, const CUtensorMap &ta, const CUtensorMap &tb,
+              int64_t clusters, int split) {
+    using Cfg = TcConfig<I8, BN, TMA>;
+    auto kernel = product_tc_kernel<I8, BN, TMA>;
+    static std::atomic<uint64_t> ready{0};  // devices whose function has its shared-memory limit raised
+    if (!(ready.load(std::memory_order_acquire) >> call.dev & 1)) {
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+        if (err != cudaSuccess) return launched(call, err);
+        ready.fetch_or(1ull << call.dev, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {static_cast<unsigned>(split), 1, 1};
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * split));
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cfg.stream = call.stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return launched(call, cudaLaunchKernelEx(&cfg, kernel, p, lay, ta, tb));
+}
+
+template <bool I8>
+int launch_product(const Call &call, const Product &p, bool bf16) {
+    constexpr int esize = I8 ? 1 : 2, bk = 128 / esize;
+    Layout lay{};
+    lay.a_mn = p.a_k != 1;
+    lay.b_mn = p.b_k != 1;
+    lay.bf16 = bf16;
+    if (p.dw) lay.a_mn = lay.b_mn = true;
+    // groups that can hold rows, and the rows of an even one
+    const int64_t groups = p.experts < p.rows ? p.experts : (p.rows ? p.rows : 1);
+    const int64_t even = (p.rows + groups - 1) / groups;
+    const int bn = p.dw ? 128 : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
+    Operand a{p.a, 0, 0, 0, 1, 0}, b{p.b, 0, 0, 0, 1, 0};
+    if (p.dw) {
+        a.inner = p.m, a.rows = p.rows, a.row_stride = p.a_k;
+        b.inner = p.c, b.rows = p.rows, b.row_stride = p.b_k;
+    } else {
+        a.inner = lay.a_mn ? p.m : p.k, a.rows = lay.a_mn ? p.k : p.m, a.row_stride = lay.a_mn ? p.a_k : p.a_m;
+        a.mats = p.experts, a.mat_stride = p.a_e;
+        b.inner = p.k, b.rows = p.rows, b.row_stride = p.b_c;
+    }
+    CUtensorMap ta{}, tb{};
+    bool tma = encode_tiled() && tma_ready(a, esize) && tma_ready(b, esize);
+    if (tma) {
+        const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                         : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+        tma = encode(&ta, a, type, esize, 3, bk, lay.a_mn ? 64 : kTileM) &&
+              encode(&tb, b, type, esize, 2, bk, lay.b_mn ? 64 : bn);
+    }
+    const int64_t mt = (p.m + kTileM - 1) / kTileM;
+    // the most tiles any grouping can have, and the tiles of an even one
+    const int64_t most = mt * (p.dw ? p.experts * ((p.c + bn - 1) / bn) : p.rows / bn + groups);
+    const int64_t tiles = p.dw ? most : mt * groups * ((even + bn - 1) / bn);
+    const int64_t kblocks = ((p.dw ? even : p.k) + bk - 1) / bk;
+    const int resident = kSms * (bn <= 32 ? 2 : 1);
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= resident && kblocks >= split * 2 * 4) split *= 2;
+    int64_t clusters = resident / split;
+    if (clusters > most) clusters = most;
+    if (!tma)
+        return bn <= 32 ? launch_tc<I8, 32, false>(call, p, lay, ta, tb, clusters, split)
+                        : launch_tc<I8, 128, false>(call, p, lay, ta, tb, clusters, split);
+    switch (bn) {
+        case 16: return launch_tc<I8, 16, true>(call, p, lay, ta, tb, clusters, split);
+        case 32: return launch_tc<I8, 32, true>(call, p, lay, ta, tb, clusters, split);
+        case 64: return launch_tc<I8, 64, true>(call, p, lay, ta, tb, clusters, split);
+        default: return launch_tc<I8, 128, true>(call, p, lay, ta, tb, clusters, split);
+    }
+}
+
+int run_product(const char *name, int dev, int operands, const Product &p, uint64_t stream) {
     if (p.m == 0 || p.experts == 0 || (p.dw ? p.c : p.rows) == 0) return EMMY_OK;
     DeviceScope scope(dev);
-    if (scope.err != cudaSuccess) return report(EMMY_ERR_CUDA, "%s: device %d: %s", name, dev, cudaGetErrorString(scope.err));
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const int64_t mt = (p.m + 63) / 64;
-    const int64_t ct = p.dw ? p.experts * ((p.c + 63) / 64) : p.rows / 64 + (p.rows < p.experts ? p.rows : p.experts);
-    const unsigned grid = static_cast<unsigned>(mt * ct < 148 * 4 ? mt * ct : 148 * 4);
-    switch (operands) {
-        case EMMY_BF16: product_simt_kernel<__nv_bfloat16, float><<<grid, 256, 0, s>>>(p); break;
-        case EMMY_F16: product_simt_kernel<__half, float><<<grid, 256, 0, s>>>(p); break;
-        default: product_simt_kernel<int8_t, int><<<grid, 256, 0, s>>>(p); break;
-    }
-    const cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return report(EMMY_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
-    return EMMY_OK;
+    if (scope.err != cudaSuccess)
+        return report(EMMY_ERR_CUDA, "%s: device %d: %s", name, dev, cudaGetErrorString(scope.err));
+    const Call call{name, dev, reinterpret_cast<cudaStream_t>(stream)};
+    return operands == kS8 ? launch_product<true>(call, p, false) : launch_product<false>(call, p, operands == EMMY_BF16);
 }
 
 int check_common(const char *name, int dev, int64_t rows, int64_t experts, int64_t n, int64_t k) {
@@ -344,7 +311,7 @@ extern "C" int emmy_grouped_matmul(int dev, int dtype, int out_dtype, const void
     p.b_c = x_stride, p.b_k = 1, p.out_c = out_stride;
     p.m = n, p.k = k, p.rows = rows;
     p.experts = static_cast<int>(experts), p.out_type = out_dtype;
-    return launch_product(name, dev, dtype, p, stream);
+    return run_product(name, dev, dtype, p, stream);
 }
 
 extern "C" int emmy_grouped_matmul_dw(int dev, int dtype, int out_dtype, const void *dy, int64_t dy_stride,
@@ -366,7 +333,7 @@ extern "C" int emmy_grouped_matmul_dw(int dev, int dtype, int out_dtype, const v
     p.b_c = 1, p.b_k = dy_stride, p.out_e = dw_stride_e, p.out_c = dw_stride_n;
     p.m = k, p.c = n, p.rows = rows;
     p.experts = static_cast<int>(experts), p.out_type = out_dtype, p.dw = true;
-    return launch_product(name, dev, dtype, p, stream);
+    return run_product(name, dev, dtype, p, stream);
 }
 
 extern "C" int emmy_int8_matmul(int dev, int out_dtype, const int8_t *xq, int64_t x_stride, const float *x_scale,
@@ -393,7 +360,7 @@ extern "C" int emmy_int8_matmul(int dev, int out_dtype, const int8_t *xq, int64_
     p.b_c = x_stride, p.b_k = 1, p.out_c = out_stride;
     p.m = n, p.k = k, p.rows = rows;
     p.experts = static_cast<int>(experts), p.out_type = out_dtype;
-    return launch_product(name, dev, kS8, p, stream);
+    return run_product(name, dev, kS8, p, stream);
 }
 
 extern "C" int emmy_quantize_rows(int dev, int dtype, const void *x, int64_t x_stride, int8_t *q, int64_t q_stride,
@@ -428,8 +395,8 @@ extern "C" int emmy_products_status(int dev, uint32_t *status) {
     cudaError_t err = scope.err;
     const unsigned int zero = 0u;
     if (err == cudaSuccess) err = cudaDeviceSynchronize();
-    if (err == cudaSuccess) err = cudaMemcpyFromSymbol(status, g_products_status, sizeof *status);
-    if (err == cudaSuccess && *status) err = cudaMemcpyToSymbol(g_products_status, &zero, sizeof zero);
+    if (err == cudaSuccess) err = cudaMemcpyFromSymbol(status, emmy_status, sizeof *status);
+    if (err == cudaSuccess && *status) err = cudaMemcpyToSymbol(emmy_status, &zero, sizeof zero);
     if (err != cudaSuccess) return report(EMMY_ERR_CUDA, "emmy_products_status: %s", cudaGetErrorString(err));
     return EMMY_OK;
 }

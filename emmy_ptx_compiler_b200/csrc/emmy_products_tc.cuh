@@ -1,0 +1,444 @@
+// Products on the 5th-generation tensor cores: out(c, m) = sum_k A(m, k) B(c, k).
+//
+// The output's contiguous axis m (the channels) lies on the 128 lanes of tensor memory and the
+// output's rows c (the tokens of a group) on the N columns of the instruction, 16 to 128 of them.
+// So a group of a few tokens costs a few columns, not a padded tile of 128 rows, and a warp's
+// 32 lanes store 32 neighbouring channels of one output row.
+#pragma once
+
+#include "emmy_products_dev.cuh"
+#include "emmy_sm100.cuh"
+
+#include <type_traits>
+
+namespace emmy {
+
+// D[tmem] (+)= A[smem] x B[smem], kind::i8, one CTA.
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// 3-D tiled load into this CTA's shared memory, completion signalled on `bar`.
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int32_t x, int32_t y,
+                                            int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// Orders this thread's plain shared-memory accesses before later ones of the async proxy (TMA, UMMA).
+__device__ __forceinline__ void fence_proxy_async() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+// Instruction descriptors: kind::f16 with either operand MN-major, and kind::i8 (s8 x s8 -> s32).
+__host__ __device__ constexpr uint32_t idesc_f16_major(uint32_t ab_fmt, uint32_t a_mn, uint32_t b_mn, uint32_t m,
+                                                       uint32_t n) {
+    return idesc_f16(ab_fmt, b_mn, m, n) | (a_mn << 15);
+}
+__host__ __device__ constexpr uint32_t idesc_s8(uint32_t m, uint32_t n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+}  // namespace emmy
+
+namespace {
+
+constexpr uint64_t kWaitNs = 2000000000ull;  // per wait: orders of magnitude above any legal one
+constexpr int kTileM = 128;
+constexpr uint32_t kBlockBytes = 128;                  // one 128-byte swizzle row of k (or of m, c)
+constexpr uint32_t kPanel = 64 * kBlockBytes;          // 64 k x 64 m (or c) of an MN-major 16-bit operand
+constexpr uint32_t kStageA = kTileM * kBlockBytes;
+
+// What a launch passes beside the product: the operands' layouts.
+struct Layout {
+    bool a_mn, b_mn;  // contiguous along m (c) instead of k
+    bool bf16;
+};
+
+struct Tile {
+    int e, begin, cols, kend, kb0, kb1;
+    int64_t m0, c0;
+};
+
+// Tile t of the launch, and the k blocks [kb0, kb1) that this CTA of the cluster sums.
+__device__ __forceinline__ Tile tile_at(const Product &p, const Groups &g, int64_t t, int64_t mt, int &e, int col_tile,
+                                        int bk, uint32_t rank, uint32_t split) {
+    while (t >= mt * g.tiles[e + 1]) ++e;
+    const int64_t r = t - mt * g.tiles[e];
+    const int begin = g.row[e], count = g.row[e + 1] - begin;
+    Tile o;
+    o.e = e;
+    o.begin = begin;
+    o.m0 = r % mt * kTileM;
+    o.c0 = r / mt * col_tile;
+    o.cols = static_cast<int>(min(static_cast<int64_t>(col_tile), (p.dw ? p.c : count) - o.c0));
+    o.kend = p.dw ? count : static_cast<int>(p.k);
+    const int nkb = o.kend / bk + (o.kend % bk != 0);
+    o.kb0 = static_cast<int>(static_cast<int64_t>(nkb) * rank / split);
+    o.kb1 = static_cast<int>(static_cast<int64_t>(nkb) * (rank + 1) / split);
+    return o;
+}
+
+// A panel of `rows` swizzled 128-byte rows from memory of any alignment: row r, byte b of it at
+// src + r * stride + b, zeros beyond the valid rows and values.  One warp of `warps`.
+template <typename T>
+__device__ __forceinline__ void load_panel(uint8_t *dst, const T *src, int64_t stride, int rows, int64_t rows_valid,
+                                           int64_t values_valid, int thread, int threads) {
+    constexpr int V = 16 / sizeof(T);
+    for (int i = thread; i < rows * 8; i += threads) {
+        const int r = i >> 3, j = i & 7;
+        alignas(16) T v[V];
+        const T *s = src + r * stride + j * V;
+        const int64_t have = r < rows_valid ? values_valid - j * V : 0;
+        if (have >= V && (reinterpret_cast<uintptr_t>(s) & 7) == 0) {
+            reinterpret_cast<uint2 *>(v)[0] = reinterpret_cast<const uint2 *>(s)[0];
+            reinterpret_cast<uint2 *>(v)[1] = reinterpret_cast<const uint2 *>(s)[1];
+        } else if (have >= V && (reinterpret_cast<uintptr_t>(s) & 3) == 0) {
+            #pragma unroll
+            for (int b = 0; b < 4; ++b) reinterpret_cast<uint32_t *>(v)[b] = reinterpret_cast<const uint32_t *>(s)[b];
+        } else {
+            #pragma unroll
+            for (int b = 0; b < V; ++b) {
+                if (b < have) v[b] = s[b];
+                else v[b] = T(0);
+            }
+        }
+        *reinterpret_cast<uint4 *>(dst + r * kBlockBytes + ((j ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4 *>(v);
+    }
+}
+
+// Rows [from, to) of a 64-row panel become zeros (whole 128-byte rows, so the swizzle does not matter).
+__device__ __forceinline__ void zero_panel_rows(uint8_t *panel, int from, int to, int lane) {
+    for (int i = from * 8 + lane; i < to * 8; i += 32) reinterpret_cast<uint4 *>(panel)[i] = make_uint4(0, 0, 0, 0);
+}
+
+template <bool I8>
+__device__ __forceinline__ float sum_value(uint32_t bits) {
+    if constexpr (I8) return __int2float_rn(static_cast<int>(bits));
+    else return __uint_as_float(bits);
+}
+
+// Scale and store one finished sum: column c of the tile, channel m.
+template <bool I8>
+__device__ __forceinline__ void finish(const Product &p, const Tile &t, int64_t m, int col, uint32_t bits, float w_scale,
+                                       float bias) {
+    float v = sum_value<I8>(bits);
+    const int64_t c = t.c0 + col;
+    if constexpr (I8) v = v * p.x_scale[t.begin + c] * w_scale + bias;
+    store_out(p.out, p.out_type, (p.dw ? t.e * p.out_e : t.begin * p.out_c) + c * p.out_c + m, v);
+}
+
+template <bool I8, int BN, bool TMA>
+struct TcConfig {
+    static constexpr uint32_t kStageB = BN * kBlockBytes;
+    static constexpr uint32_t kStage = kStageA + kStageB;
+    static constexpr uint32_t kRed = BN * kTileM * 4;  // partial sums for the cluster
+    static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
+    static constexpr int kThreads = TMA ? 192 : 320;
+    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + 256;
+    static constexpr uint32_t kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
+};
+
+// Warp 0 loads operand tiles by TMA (TMA false: warps 6 to 9 do, with plain loads, for addresses
+// TMA cannot take), warp 1 issues the MMAs into one of two accumulators, warps 2 to 5 turn the
+// other into output.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
+// added in rank order through distributed shared memory, each CTA finishing its share of columns:
+// the result depends on neither timing nor the number of SMs.
+template <bool I8, int BN, bool TMA>
+__global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
+    product_tc_kernel(const Product p, const Layout lay, const __grid_constant__ CUtensorMap tm_a,
+                      const __grid_constant__ CUtensorMap tm_b) {
+    using Cfg = TcConfig<I8, BN, TMA>;
+    using T = std::conditional_t<I8, int8_t, uint16_t>;
+    constexpr int STAGES = Cfg::kStages;
+    constexpr int BK = I8 ? 128 : 64;
+    constexpr uint32_t LOADERS = TMA ? 1 : 4;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ Groups g;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem;
+    uint8_t *sB = sA + STAGES * kStageA;
+    uint32_t *red = reinterpret_cast<uint32_t *>(sB + STAGES * Cfg::kStageB);
+    uint64_t *full = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(red) + Cfg::kRed);
+    uint64_t *empty = full + STAGES;
+    uint64_t *tfull = empty + STAGES;
+    uint64_t *tempty = tfull + 2;
+    uint64_t *drain = tempty + 2;
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile uint32_t *abort_flag = tmem_holder + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = emmy::cluster_ctarank(), split = emmy::cluster_nctarank();
+
+    if (threadIdx.x == 64) {
+        for (int s = 0; s < STAGES; ++s) {
+            emmy::mbar_init(&full[s], LOADERS);
+            emmy::mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            emmy::mbar_init(&tfull[a], 1);
+            emmy::mbar_init(&tempty[a], 4);
+        }
+        emmy::mbar_init(drain, 1);
+        *abort_flag = 0u;
+        emmy::fence_barrier_init();
+    }
+    if (warp == 1) {
+        emmy::tmem_alloc(tmem_holder, Cfg::kTmemCols);
+        emmy::tmem_relinquish();
+    }
+    if (warp == 0) {
+        if (TMA && lane == 0) {
+            emmy::tma_prefetch(&tm_a);
+            emmy::tma_prefetch(&tm_b);
+        }
+        load_groups(g, p, BN);
+    }
+    emmy::tc_fence_before();
+    __syncthreads();
+    emmy::tc_fence_after();
+    const uint32_t tmem_base = *tmem_holder;
+
+    const int64_t mt = (p.m + kTileM - 1) / kTileM, total = mt * g.tiles[p.experts];
+    const int64_t step = gridDim.x / split;
+    uint32_t stage = 0, phase = 0, it = 0;
+    uint32_t issued = 0u, parity_bits = 0u;  // producer: loads in flight for each stage and their parity
+    bool ok = true;
+    int e = 0;
+    // Without a cluster each role runs through all of the CTA's tiles at its own pace; a cluster
+    // takes one tile at a time, because its CTAs meet after each.
+    for (int64_t first = blockIdx.x / split; first < total; first += split > 1 ? step : total) {
+        const int64_t last = split > 1 ? first + 1 : total;
+        if (TMA && warp == 0) {
+            if (lane == 0) {
+                for (int64_t t = first; t < last && ok; t += step) {
+                    const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
+                    const int m0 = static_cast<int>(w.m0), c0 = static_cast<int>(w.c0);
+                    for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                        if (!emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
+                            ok = false;
+                            break;
+                        }
+                        emmy::mbar_arrive_expect_tx(&full[stage], Cfg::kStage);
+                        uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
+                        const int k0 = kb * BK;
+                        if (lay.a_mn) {
+                            const int ka = p.dw ? w.begin + k0 : k0, ez = p.dw ? 0 : w.e;
+                            emmy::tma_load_3d(a, &tm_a, &full[stage], m0, ka, ez);
+                            emmy::tma_load_3d(a + kPanel, &tm_a, &full[stage], m0 + 64, ka, ez);
+                        } else {
+                            emmy::tma_load_3d(a, &tm_a, &full[stage], k0, m0, w.e);
+                        }
+                        if (lay.b_mn) {
+                            for (int j = 0; j < BN / 64; ++j)
+                                emmy::tma_load_2d(b + j * kPanel, &tm_b, &full[stage], c0 + 64 * j, w.begin + k0);
+                        } else {
+                            emmy::tma_load_2d(b, &tm_b, &full[stage], k0, w.begin + c0);
+                        }
+                        issued |= 1u << stage;
+                        parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+        } else if (!TMA && warp >= 6) {
+            const int th = threadIdx.x - 192;
+            for (int64_t t = first; t < last && ok; t += step) {
+                const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
+                const T *ae = static_cast<const T *>(p.a) + (p.dw ? w.begin * p.a_k : w.e * p.a_e);
+                const T *be = static_cast<const T *>(p.b) + w.begin * (p.dw ? p.b_k : p.b_c);
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    if (!emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
+                    const int64_t k0 = static_cast<int64_t>(kb) * BK;
+                    if (lay.a_mn) {
+                        for (int j = 0; j < 2; ++j)
+                            load_panel(a + j * kPanel, ae + k0 * p.a_k + w.m0 + 64 * j, p.a_k, 64, w.kend - k0,
+                                       p.m - w.m0 - 64 * j, th, 128);
+                    } else {
+                        load_panel(a, ae + w.m0 * p.a_m + k0, p.a_m, kTileM, p.m - w.m0, w.kend - k0, th, 128);
+                    }
+                    if (lay.b_mn) {
+                        for (int j = 0; j < BN / 64; ++j)
+                            load_panel(b + j * kPanel, be + k0 * p.b_k + w.c0 + 64 * j, p.b_k, 64, w.kend - k0,
+                                       w.cols - 64 * j, th, 128);
+                    } else {
+                        load_panel(b, be + w.c0 * p.b_c + k0, p.b_c, BN, w.cols, w.kend - k0, th, 128);
+                    }
+                    emmy::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) emmy::mbar_arrive(&full[stage]);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            const uint32_t idesc = I8 ? emmy::idesc_s8(kTileM, BN)
+                                      : emmy::idesc_f16_major(lay.bf16 ? 1u : 0u, lay.a_mn, lay.b_mn, kTileM, BN);
+            // one MMA takes 32 bytes of k: along a swizzled row when k is contiguous, else 16 rows further
+            const uint32_t a_step = lay.a_mn ? 16 * kBlockBytes : 32, a_lbo = lay.a_mn ? kPanel : 16;
+            const uint32_t b_step = lay.b_mn ? 16 * kBlockBytes : 32, b_lbo = lay.b_mn ? kPanel : 16;
+            for (int64_t t = first; t < last && ok; t += step, ++it) {
+                const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
+                const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
+                if (!emmy::mbar_wait(&tempty[acc], aphase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) {
+                    ok = false;
+                    break;
+                }
+                emmy::tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * BN;
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    if (!emmy::mbar_wait(&full[stage], phase, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
+                    int steps = 4;
+                    if (p.dw && w.kend - kb * BK < BK) {
+                        // the block ends inside: later rows belong to the next group (or hold
+                        // anything), so what the last MMA takes of them becomes zero in both operands
+                        const int have = w.kend - kb * BK;
+                        steps = (have + 15) / 16;
+                        if (TMA) {
+                            for (int j = 0; j < 2; ++j) zero_panel_rows(a + j * kPanel, have, steps * 16, lane);
+                            for (int j = 0; j < BN / 64; ++j) zero_panel_rows(b + j * kPanel, have, steps * 16, lane);
+                            emmy::fence_proxy_async();
+                            __syncwarp();
+                        }
+                    }
+                    emmy::tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t a_base = emmy::smem_u32(a), b_base = emmy::smem_u32(b);
+                        for (int kk = 0; kk < steps; ++kk) {
+                            const uint64_t ad = emmy::smem_desc_sw128(a_base + kk * a_step, a_lbo, 1024);
+                            const uint64_t bd = emmy::smem_desc_sw128(b_base + kk * b_step, b_lbo, 1024);
+                            const uint32_t more = (kb > w.kb0 || kk > 0) ? 1u : 0u;
+                            if constexpr (I8) emmy::umma_i8(d_tmem, ad, bd, idesc, more);
+                            else emmy::umma_f16(d_tmem, ad, bd, idesc, more);
+                        }
+                        emmy::umma_commit(&empty[stage]);
+                    }
+                    __syncwarp();
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                if (lane == 0) emmy::umma_commit(&tfull[acc]);
+                __syncwarp();
+            }
+        } else if (warp >= 2 && warp < 6) {
+            const int q = warp & 3;
+            for (int64_t t = first; t < last && ok; t += step, ++it) {
+                const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
+                const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
+                if (!emmy::mbar_wait(&tfull[acc], aphase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)) {
+                    ok = false;
+                    break;
+                }
+                emmy::tc_fence_after();
+                const int64_t m = w.m0 + q * 32 + lane;
+                float w_scale = 0.0f, bias = 0.0f;
+                if (I8 && split == 1 && m < p.m) {
+                    w_scale = p.w_scale[w.e * p.m + m];
+                    if (p.bias) bias = p.bias[w.e * p.m + m];
+                }
+                #pragma unroll 1
+                for (int c = 0; c < w.cols; c += 16) {
+                    uint32_t r[16];
+                    emmy::tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN + c, r);
+                    emmy::tmem_ld_wait();
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (c + j >= w.cols) break;
+                        const uint32_t v = w.kb0 < w.kb1 ? r[j] : 0u;  // no k: nothing was accumulated
+                        if (split > 1) red[(c + j) * kTileM + q * 32 + lane] = v;
+                        else if (m < p.m) finish<I8>(p, w, m, c + j, v, w_scale, bias);
+                    }
+                }
+                emmy::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) emmy::mbar_arrive(&tempty[acc]);
+            }
+        }
+        if (split > 1) {
+            __syncwarp();
+            emmy::cluster_sync();  // every CTA's partial sums are in its shared memory
+            if (warp >= 2 && warp < 6 && ok) {
+                const Tile w = tile_at(p, g, first, mt, e, BN, BK, rank, split);
+                const int lm = (warp & 3) * 32 + lane;
+                const int64_t m = w.m0 + lm;
+                if (m < p.m) {
+                    float w_scale = 0.0f, bias = 0.0f;
+                    if (I8) {
+                        w_scale = p.w_scale[w.e * p.m + m];
+                        if (p.bias) bias = p.bias[w.e * p.m + m];
+                    }
+                    for (int c = rank; c < w.cols; c += split) {
+                        uint32_t sum = 0u;  // 0 of either type
+                        for (uint32_t s = 0; s < split; ++s) {
+                            const uint32_t v = emmy::ld_cluster_u32(emmy::mapa(&red[c * kTileM + lm], s));
+                            sum = I8 ? sum + v : __float_as_uint(__uint_as_float(sum) + __uint_as_float(v));
+                        }
+                        finish<I8>(p, w, m, c, sum, w_scale, bias);
+                    }
+                }
+            }
+            __syncwarp();
+            emmy::cluster_sync();  // and may be overwritten
+        }
+    }
+
+    if (TMA && warp == 0 && lane == 0 && !ok) {
+        // this CTA's own loads still in flight land before it leaves (bounded)
+        volatile uint32_t never = 0u;
+        for (int s = 0; s < STAGES; ++s)
+            if (issued & (1u << s)) emmy::mbar_wait(&full[s], (parity_bits >> s) & 1u, &never, 0u, 20000000ull);
+    }
+    if (warp == 1 && lane == 0) {
+        // every MMA has finished before tensor memory is released (bounded)
+        emmy::umma_commit(drain);
+        volatile uint32_t never = 0u;
+        emmy::mbar_wait(drain, 0u, &never, 0u, 20000000ull);
+    }
+    emmy::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        emmy::tc_fence_after();
+        emmy::tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+}
+
+}  // namespace

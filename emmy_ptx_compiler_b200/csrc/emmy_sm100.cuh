@@ -18,7 +18,9 @@
 
 #include "emmy_launch_record.h"
 
+#ifndef EMMY_STATUS_DEFINED  // a file whose status word is private to it defines the word first
 extern "C" __device__ unsigned int emmy_status;
+#endif
 
 namespace emmy {
 

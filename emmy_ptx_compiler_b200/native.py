@@ -21,7 +21,8 @@ SOURCES = [PKG / "csrc" / "emmy_runtime.cpp"]
 CUDA_SOURCES = [PKG / "csrc" / "emmy_noalloc.cu", PKG / "csrc" / "emmy_xchg.cu",
                 PKG / "csrc" / "emmy_products.cu"]
 HEADERS = [REPO / "include" / "emmy_b200.h", REPO / "include" / "emmy_launch_record.h",
-           PKG / "csrc" / "emmy_xchg_dev.cuh", PKG / "csrc" / "emmy_sm100.cuh"]
+           PKG / "csrc" / "emmy_xchg_dev.cuh", PKG / "csrc" / "emmy_sm100.cuh",
+           PKG / "csrc" / "emmy_products_dev.cuh", PKG / "csrc" / "emmy_products_tc.cuh"]
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 CUDA_INC = CUDA_HOME / "include"
 CUDA_LIB = CUDA_HOME / "lib64"
