@@ -189,42 +189,58 @@ int launched(const Call &call, cudaError_t err) {
     return report(EMMY_ERR_CUDA, "%s: launch: %s", call.name, cudaGetErrorString(err));
 }
 
-template <bool I8, int BN, bool TMA>
-int launch_tc(const Call &call, const Product &p, const Layout &lay, const CUtensorMap &ta, const CUtensorMap &tb,
-              int64_t clusters, int split) {
-    using Cfg = TcConfig<I8, BN, TMA>;
-    auto kernel = product_tc_kernel<I8, BN, TMA>;
-    static std::atomic<uint64_t> ready{0};  // devices whose function has its shared-memory limit raised
+using TcKernel = void (*)(Product, Layout, CUtensorMap, CUtensorMap);
+
+// A launch of clusters of `cluster` CTAs.  `ready` marks the devices on which the kernel's
+// shared-memory limit has been raised.
+int launch_clusters(const Call &call, TcKernel kernel, std::atomic<uint64_t> &ready, const Product &p, const Layout &lay,
+                    const CUtensorMap &ta, const CUtensorMap &tb, int64_t clusters, int cluster, int threads,
+                    uint32_t smem) {
     if (!(ready.load(std::memory_order_acquire) >> call.dev & 1)) {
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+        const cudaError_t err =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (err != cudaSuccess) return launched(call, err);
         ready.fetch_or(1ull << call.dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {static_cast<unsigned>(split), 1, 1};
-    cfg.gridDim = dim3(static_cast<unsigned>(clusters * split));
-    cfg.blockDim = dim3(Cfg::kThreads);
-    cfg.dynamicSmemBytes = Cfg::kSmem;
+    attr.val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = call.stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     return launched(call, cudaLaunchKernelEx(&cfg, kernel, p, lay, ta, tb));
 }
 
+template <bool I8, int BN, bool TMA>
+int launch_single(const Call &call, const Product &p, const Layout &lay, const CUtensorMap &ta, const CUtensorMap &tb,
+                  int64_t clusters, int split) {
+    using Cfg = TcConfig<I8, BN, TMA>;
+    static std::atomic<uint64_t> ready{0};
+    return launch_clusters(call, product_tc_kernel<I8, BN, TMA>, ready, p, lay, ta, tb, clusters, split, Cfg::kThreads,
+                           Cfg::kSmem);
+}
+
+template <bool I8, int BN>
+int launch_pair(const Call &call, const Product &p, const Layout &lay, const CUtensorMap &ta, const CUtensorMap &tb,
+                int64_t pairs) {
+    static std::atomic<uint64_t> ready{0};
+    return launch_clusters(call, product_pair_kernel<I8, BN>, ready, p, lay, ta, tb, pairs, 2, 192,
+                           PairConfig<BN>::kSmem);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 template <bool I8>
 int launch_product(const Call &call, const Product &p, bool bf16) {
     constexpr int esize = I8 ? 1 : 2, bk = 128 / esize;
     Layout lay{};
-    lay.a_mn = p.a_k != 1;
-    lay.b_mn = p.b_k != 1;
+    lay.a_mn = p.dw || p.a_k != 1;
+    lay.b_mn = p.dw;
     lay.bf16 = bf16;
-    if (p.dw) lay.a_mn = lay.b_mn = true;
-    // groups that can hold rows, and the rows of an even one
-    const int64_t groups = p.experts < p.rows ? p.experts : (p.rows ? p.rows : 1);
-    const int64_t even = (p.rows + groups - 1) / groups;
-    const int bn = p.dw ? 128 : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
     Operand a{p.a, 0, 0, 0, 1, 0}, b{p.b, 0, 0, 0, 1, 0};
     if (p.dw) {
         a.inner = p.m, a.rows = p.rows, a.row_stride = p.a_k;
@@ -234,33 +250,54 @@ int launch_product(const Call &call, const Product &p, bool bf16) {
         a.mats = p.experts, a.mat_stride = p.a_e;
         b.inner = p.k, b.rows = p.rows, b.row_stride = p.b_c;
     }
-    CUtensorMap ta{}, tb{};
     bool tma = encode_tiled() && tma_ready(a, esize) && tma_ready(b, esize);
+
+    // groups that can hold rows, and the rows of an even one
+    const int64_t groups = p.experts < p.rows ? p.experts : (p.rows ? p.rows : 1);
+    const int64_t even = ceil_div(p.rows, groups), kblocks = ceil_div(p.dw ? even : p.k, bk);
+    // tiles of even groups, and the most that any grouping can have
+    auto tiles = [&](int64_t tm, int64_t tc) {
+        return ceil_div(p.m, tm) * (p.dw ? p.experts * ceil_div(p.c, tc) : groups * ceil_div(even, tc));
+    };
+    auto most = [&](int64_t tm, int64_t tc) {
+        return ceil_div(p.m, tm) * (p.dw ? p.experts * ceil_div(p.c, tc) : p.rows / tc + groups);
+    };
+    const int64_t cext = p.dw ? p.c : even;
+    int pair = 0;
+    if (tma && p.m > 128 && cext > 64) {
+        if (cext > 192 && tiles(256, 256) >= kSms / 4) pair = 256;
+        else if (tiles(256, 128) >= kSms / 4) pair = 128;
+    }
+    const int bn = pair ? pair : p.dw ? 128 : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
+
+    CUtensorMap ta{}, tb{};
     if (tma) {
         const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                          : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-        tma = encode(&ta, a, type, esize, 3, bk, lay.a_mn ? 64 : kTileM) &&
-              encode(&tb, b, type, esize, 2, bk, lay.b_mn ? 64 : bn);
+        if (!encode(&ta, a, type, esize, 3, bk, lay.a_mn ? 64 : kTileM) ||
+            !encode(&tb, b, type, esize, 2, bk, lay.b_mn ? 64 : pair ? pair / 2 : bn))
+            return report(EMMY_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", call.name);
     }
-    const int64_t mt = (p.m + kTileM - 1) / kTileM;
-    // the most tiles any grouping can have, and the tiles of an even one
-    const int64_t most = mt * (p.dw ? p.experts * ((p.c + bn - 1) / bn) : p.rows / bn + groups);
-    const int64_t tiles = p.dw ? most : mt * groups * ((even + bn - 1) / bn);
-    const int64_t kblocks = ((p.dw ? even : p.k) + bk - 1) / bk;
+    if (pair) {
+        int64_t pairs = most(256, pair);
+        if (pairs > kSms / 2) pairs = kSms / 2;
+        return pair == 256 ? launch_pair<I8, 256>(call, p, lay, ta, tb, pairs)
+                           : launch_pair<I8, 128>(call, p, lay, ta, tb, pairs);
+    }
     const int resident = kSms * (bn <= 32 ? 2 : 1);
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= resident && kblocks >= split * 2 * 4) split *= 2;
-    int64_t clusters = resident / split;
-    if (clusters > most) clusters = most;
+    while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident && kblocks >= split * 2 * 4) split *= 2;
+    int64_t clusters = most(kTileM, bn);
+    if (clusters > resident / split) clusters = resident / split;
     if (!tma)
-        return bn <= 32 ? launch_tc<I8, 32, false>(call, p, lay, ta, tb, clusters, split)
-                        : launch_tc<I8, 128, false>(call, p, lay, ta, tb, clusters, split);
+        return bn <= 32 ? launch_single<I8, 32, false>(call, p, lay, ta, tb, clusters, split)
+                        : launch_single<I8, 128, false>(call, p, lay, ta, tb, clusters, split);
     switch (bn) {
-        case 16: return launch_tc<I8, 16, true>(call, p, lay, ta, tb, clusters, split);
-        case 32: return launch_tc<I8, 32, true>(call, p, lay, ta, tb, clusters, split);
-        case 64: return launch_tc<I8, 64, true>(call, p, lay, ta, tb, clusters, split);
-        default: return launch_tc<I8, 128, true>(call, p, lay, ta, tb, clusters, split);
+        case 16: return launch_single<I8, 16, true>(call, p, lay, ta, tb, clusters, split);
+        case 32: return launch_single<I8, 32, true>(call, p, lay, ta, tb, clusters, split);
+        case 64: return launch_single<I8, 64, true>(call, p, lay, ta, tb, clusters, split);
+        default: return launch_single<I8, 128, true>(call, p, lay, ta, tb, clusters, split);
     }
 }
 

@@ -33,6 +33,45 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
         : "r"(taddr));
 }
 
+// 16 lanes x 32 consecutive 32-bit columns in matrix-fragment order: register 4 g + i of thread t
+// holds lane t / 4 + 8 (i / 2) and column 8 g + 2 (t % 4) + i % 2.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// Four 8 x 8 matrices of 16-bit values in fragment order, stored transposed: lane 8 i + j gives the
+// address of column j of matrix i.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t smem_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_addr), "r"(a),
+                 "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+
+// D[tmem of both CTAs] (+)= A x B over both CTAs' shared memory, kind::i8; issued by the leader.
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 3-D tiled load into this CTA's shared memory, completion counted on the mbarrier at
+// shared::cluster address `bar_cluster` (the leader's).
+__device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *map, uint32_t bar_cluster, int32_t x,
+                                                 int32_t y, int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
 // 3-D tiled load into this CTA's shared memory, completion signalled on `bar`.
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int32_t x, int32_t y,
                                             int32_t z) {
@@ -149,6 +188,108 @@ __device__ __forceinline__ void finish(const Product &p, const Tile &t, int64_t 
     const int64_t c = t.c0 + col;
     if constexpr (I8) v = v * p.x_scale[t.begin + c] * w_scale + bias;
     store_out(p.out, p.out_type, (p.dw ? t.e * p.out_e : t.begin * p.out_c) + c * p.out_c + m, v);
+}
+
+// Staging of a warp's 32 channels x 32 output rows: 64 bytes a row, 80 apart, so that neither the
+// transposed 8 x 8 stores nor the 16-byte reads meet bank conflicts.
+constexpr uint32_t kStoreRow = 80, kStoreBytes = 32 * kStoreRow;
+
+__device__ __forceinline__ uint32_t pack16(bool bf16, float lo, float hi) {
+    if (bf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// The accumulator's channels lie on lanes, the output's along a row.  16-bit outputs are transposed
+// on the way: fragments of 8 x 8 go to shared memory through stmatrix, and 4 lanes then write each
+// 64-byte piece of an output row 16 bytes at a time (8 stores a block instead of 32, and the
+// conversion packs two values).  f32 outputs need no help: 32 lanes write 128 bytes of a row.
+template <bool I8>
+__device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int64_t mq, uint32_t taddr, bool empty,
+                                           uint8_t *buf, int lane) {
+    if (p.out_type == EMMY_F32) {
+        const int64_t m = mq + lane;
+        float ws = 0.0f, bias = 0.0f;
+        if (I8 && m < p.m) {
+            ws = p.w_scale[w.e * p.m + m];
+            if (p.bias) bias = p.bias[w.e * p.m + m];
+        }
+        #pragma unroll 1
+        for (int c = 0; c < w.cols; c += 16) {
+            uint32_t r[16];
+            emmy::tmem_ld_32x32b_x16(taddr + c, r);
+            emmy::tmem_ld_wait();
+            if (m < p.m) {
+                #pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (c + j < w.cols) finish<I8>(p, w, m, c + j, empty ? 0u : r[j], ws, bias);
+            }
+        }
+        return;
+    }
+    uint16_t *out = static_cast<uint16_t *>(p.out) +
+                    ((p.dw ? w.e * p.out_e : w.begin * p.out_c) + w.c0 * p.out_c + mq);
+    const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && ((p.out_c | p.out_e | p.m) & 7) == 0;
+    const bool bf16 = p.out_type == EMMY_BF16;
+    float ws[4] = {}, bias[4] = {};
+    if constexpr (I8) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t m = mq + lane / 4 + 8 * i;
+            if (m < p.m) {
+                ws[i] = p.w_scale[w.e * p.m + m];
+                if (p.bias) bias[i] = p.bias[w.e * p.m + m];
+            }
+        }
+    }
+    #pragma unroll 1
+    for (int c = 0; c < w.cols; c += 32) {
+        float xs[8];
+        if constexpr (I8) {
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int col = c + 8 * (i >> 1) + 2 * (lane & 3) + (i & 1);
+                xs[i] = col < w.cols ? p.x_scale[w.begin + w.c0 + col] : 0.0f;
+            }
+        }
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t r[16], v[8];
+            emmy::tmem_ld_16x256b_x4(taddr + (static_cast<uint32_t>(16 * h) << 16) + c, r);
+            emmy::tmem_ld_wait();
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float lo = sum_value<I8>(empty ? 0u : r[2 * i]), hi = sum_value<I8>(empty ? 0u : r[2 * i + 1]);
+                if constexpr (I8) {
+                    const int row = 2 * h + (i & 1);
+                    lo = lo * xs[i >> 1 << 1] * ws[row] + bias[row];
+                    hi = hi * xs[(i >> 1 << 1) + 1] * ws[row] + bias[row];
+                }
+                v[i] = pack16(bf16, lo, hi);
+            }
+            const uint32_t at = emmy::smem_u32(buf) + ((lane >> 4) * 8 + (lane & 7)) * kStoreRow +
+                                (16 * h + 8 * ((lane >> 3) & 1)) * 2;
+            emmy::stmatrix_x4_trans(at, v[0], v[1], v[2], v[3]);
+            emmy::stmatrix_x4_trans(at + 16 * kStoreRow, v[4], v[5], v[6], v[7]);
+        }
+        __syncwarp();
+        if (vec) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = i * 8 + (lane >> 2), piece = lane & 3;
+                if (c + row < w.cols && mq + piece * 8 < p.m)
+                    *reinterpret_cast<uint4 *>(out + (c + row) * p.out_c + piece * 8) =
+                        *reinterpret_cast<const uint4 *>(buf + row * kStoreRow + piece * 16);
+            }
+        } else if (mq + lane < p.m) {
+            for (int row = 0; row < 32 && c + row < w.cols; ++row)
+                out[(c + row) * p.out_c + lane] = *reinterpret_cast<const uint16_t *>(buf + row * kStoreRow + lane * 2);
+        }
+        __syncwarp();
+    }
 }
 
 template <bool I8, int BN, bool TMA>
@@ -371,6 +512,15 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                 emmy::tc_fence_after();
                 const int64_t m = w.m0 + q * 32 + lane;
                 float w_scale = 0.0f, bias = 0.0f;
+                if (BN >= 64 && split == 1) {
+                    // the sums' exchange buffer is free without a cluster
+                    store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN,
+                                   w.kb0 == w.kb1, reinterpret_cast<uint8_t *>(red) + q * kStoreBytes, lane);
+                    emmy::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) emmy::mbar_arrive(&tempty[acc]);
+                    continue;
+                }
                 if (I8 && split == 1 && m < p.m) {
                     w_scale = p.w_scale[w.e * p.m + m];
                     if (p.bias) bias = p.bias[w.e * p.m + m];
@@ -438,6 +588,259 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
     if (warp == 1) {
         emmy::tc_fence_after();
         emmy::tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------- CTA pairs
+//
+// For groups of many rows: 256 channels x BN rows of output on a pair of CTAs.  Each CTA loads its
+// 128 channels of A and its half of B's rows, the leader issues cta_group::2 MMAs over both CTAs'
+// shared memory, and each CTA turns its own 128 lanes into output while the next tile accumulates.
+// A pair moves 64 bytes into shared memory per SM and clock of MMA (BN = 256), half of what a
+// single CTA's 128 x 128 tile needs - more than L2 delivers.
+
+template <int BN>
+struct PairConfig {
+    static constexpr uint32_t kStageB = BN / 2 * kBlockBytes;
+    static constexpr uint32_t kStage = kStageA + kStageB;
+    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr uint32_t kSmem = 1024 + kStages * kStage + 4 * kStoreBytes + 256;
+    static constexpr int kSweep = 8;  // channel tiles that share one sweep over a group's rows
+};
+
+template <bool I8, int BN>
+__global__ void __launch_bounds__(192, 1)
+    product_pair_kernel(const Product p, const Layout lay, const __grid_constant__ CUtensorMap tm_a,
+                        const __grid_constant__ CUtensorMap tm_b) {
+    using Cfg = PairConfig<BN>;
+    constexpr int STAGES = Cfg::kStages, BK = I8 ? 128 : 64, CN = BN / 2;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ Groups g;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem;
+    uint8_t *sB = sA + STAGES * kStageA;
+    uint8_t *sStore = sB + STAGES * Cfg::kStageB;
+    uint64_t *full = reinterpret_cast<uint64_t *>(sStore + 4 * kStoreBytes);
+    uint64_t *empty = full + STAGES;
+    uint64_t *tfull = empty + STAGES;
+    uint64_t *tempty = tfull + 2;
+    uint64_t *drain = tempty + 2;
+    uint64_t *tail = drain + 1;       // this CTA's loads of a block that ends inside
+    // the peer's are in and their spare rows zeroed (leader only); one for each stage, because the
+    // peer may be several blocks ahead, but never twice on one stage
+    uint64_t *tail_peer = tail + 1;
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(tail_peer + STAGES);
+    volatile uint32_t *abort_flag = tmem_holder + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = emmy::cluster_ctarank();
+
+    if (threadIdx.x == 64) {
+        for (int s = 0; s < STAGES; ++s) {
+            emmy::mbar_init(&full[s], 1);
+            emmy::mbar_init(&empty[s], 1);
+            emmy::mbar_init(&tail_peer[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            emmy::mbar_init(&tfull[a], 1);
+            emmy::mbar_init(&tempty[a], 8);
+        }
+        emmy::mbar_init(drain, 1);
+        emmy::mbar_init(tail, 1);
+        *abort_flag = 0u;
+        emmy::fence_barrier_init();
+    }
+    if (warp == 1) {
+        emmy::tmem_alloc_pair(tmem_holder, 2 * BN);
+        emmy::tmem_relinquish_pair();
+    }
+    if (warp == 0) {
+        if (lane == 0) {
+            emmy::tma_prefetch(&tm_a);
+            emmy::tma_prefetch(&tm_b);
+        }
+        load_groups(g, p, BN);
+    }
+    emmy::tc_fence_before();
+    __syncthreads();
+    emmy::cluster_sync();  // the peer signals the leader's barriers only after both are initialised
+    emmy::tc_fence_after();
+    const uint32_t tmem_base = *tmem_holder;
+    const int64_t mt = (p.m + 2 * kTileM - 1) / (2 * kTileM), total = mt * g.tiles[p.experts];
+    const int64_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    int e = 0;
+
+    // Tile t: within an expert, kSweep channel tiles go over all of its rows together.
+    auto tile = [&](int64_t t) {
+        while (t >= mt * g.tiles[e + 1]) ++e;
+        const int begin = g.row[e], count = g.row[e + 1] - begin;
+        const int64_t ct = g.tiles[e + 1] - g.tiles[e], r = t - mt * g.tiles[e];
+        const int64_t sweep = r / (Cfg::kSweep * ct), in = r - sweep * Cfg::kSweep * ct;
+        const int64_t first = sweep * Cfg::kSweep, wide = min(static_cast<int64_t>(Cfg::kSweep), mt - first);
+        Tile o;
+        o.e = e;
+        o.begin = begin;
+        o.m0 = (first + in % wide) * 2 * kTileM + rank * kTileM;
+        o.c0 = in / wide * BN;
+        o.cols = static_cast<int>(min(static_cast<int64_t>(BN), (p.dw ? p.c : count) - o.c0));
+        o.kend = p.dw ? count : static_cast<int>(p.k);
+        o.kb0 = 0;
+        o.kb1 = o.kend / BK + (o.kend % BK != 0);
+        return o;
+    };
+
+    if (warp == 0) {
+        // ---------------- loads (both CTAs; completion counted on the leader's barrier)
+        uint32_t stage = 0, phase = 0, tails = 0;
+        uint32_t peer_parity = 0u;  // of tail_peer, one bit for each stage
+        uint32_t issued = 0u, parity_bits = 0u;
+        bool ok = true;
+        for (int64_t t = pair; t < total && ok; t += npairs) {
+            const Tile w = tile(t);
+            const int m0 = static_cast<int>(w.m0), c0 = static_cast<int>(w.c0) + static_cast<int>(rank) * CN;
+            for (int kb = 0; kb < w.kb1; ++kb) {
+                if (!emmy::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
+                const int k0 = kb * BK, have = w.kend - k0;
+                const bool ends_inside = p.dw && have < BK;
+                if (lane == 0) {
+                    if (ends_inside) emmy::mbar_arrive_expect_tx(tail, Cfg::kStage);
+                    else if (rank == 0) emmy::mbar_arrive_expect_tx(&full[stage], 2u * Cfg::kStage);
+                    const uint32_t bar = ends_inside ? emmy::mapa(tail, rank) : emmy::mapa(&full[stage], 0);
+                    if (lay.a_mn) {
+                        const int ka = p.dw ? w.begin + k0 : k0, ez = p.dw ? 0 : w.e;
+                        emmy::tma_load_3d_pair(a, &tm_a, bar, m0, ka, ez);
+                        emmy::tma_load_3d_pair(a + kPanel, &tm_a, bar, m0 + 64, ka, ez);
+                    } else {
+                        emmy::tma_load_3d_pair(a, &tm_a, bar, k0, m0, w.e);
+                    }
+                    if (lay.b_mn) {
+                        for (int j = 0; j < CN / 64; ++j)
+                            emmy::tma_load_2d_pair(b + j * kPanel, &tm_b, bar, c0 + 64 * j, w.begin + k0);
+                    } else {
+                        emmy::tma_load_2d_pair(b, &tm_b, bar, k0, w.begin + c0);
+                    }
+                }
+                __syncwarp();
+                if (ends_inside) {
+                    // later rows belong to the next group (or hold anything): what the last MMA takes
+                    // of them becomes zero in both operands before the leader's barrier completes
+                    ok = emmy::mbar_wait_cluster(tail, tails & 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const int upto = (have + 15) / 16 * 16;
+                    for (int j = 0; j < 2; ++j) zero_panel_rows(a + j * kPanel, have, upto, lane);
+                    for (int j = 0; j < CN / 64; ++j) zero_panel_rows(b + j * kPanel, have, upto, lane);
+                    emmy::fence_proxy_async();
+                    __syncwarp();
+                    if (rank == 1) {
+                        if (lane == 0) emmy::mbar_arrive_cluster(emmy::mapa(&tail_peer[stage], 0));
+                    } else {
+                        ok = emmy::mbar_wait_cluster(&tail_peer[stage], peer_parity >> stage & 1u, abort_flag,
+                                                     EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
+                        peer_parity ^= 1u << stage;
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0) emmy::mbar_arrive(&full[stage]);
+                    }
+                    ++tails;
+                } else if (rank == 0) {
+                    issued |= 1u << stage;
+                    parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
+                }
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok && rank == 0 && lane == 0) {
+            // loads still in flight land before the pair leaves (bounded)
+            volatile uint32_t never = 0u;
+            for (int s = 0; s < STAGES; ++s)
+                if (issued & (1u << s)) emmy::mbar_wait_cluster(&full[s], (parity_bits >> s) & 1u, &never, 0u, 20000000ull);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0 && lane == 0) {
+            // ---------------- MMA issuer (leader only)
+            const uint32_t idesc = I8 ? emmy::idesc_s8(2 * kTileM, BN)
+                                      : emmy::idesc_f16_major(lay.bf16 ? 1u : 0u, lay.a_mn, lay.b_mn, 2 * kTileM, BN);
+            const uint32_t a_step = lay.a_mn ? 16 * kBlockBytes : 32, a_lbo = lay.a_mn ? kPanel : 16;
+            const uint32_t b_step = lay.b_mn ? 16 * kBlockBytes : 32, b_lbo = lay.b_mn ? kPanel : 16;
+            const uint32_t peer_empty = emmy::mapa(&empty[0], 1);
+            uint32_t stage = 0, phase = 0, it = 0;
+            bool ok = true;
+            for (int64_t t = pair; t < total && ok; t += npairs, ++it) {
+                const Tile w = tile(t);
+                const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
+                if (!emmy::mbar_wait_cluster(&tempty[acc], aphase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) break;
+                emmy::tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * BN;
+                for (int kb = 0; kb < w.kb1; ++kb) {
+                    if (!emmy::mbar_wait_cluster(&full[stage], phase, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) {
+                        ok = false;
+                        break;
+                    }
+                    emmy::tc_fence_after();
+                    const uint32_t a_base = emmy::smem_u32(sA + stage * kStageA);
+                    const uint32_t b_base = emmy::smem_u32(sB + stage * Cfg::kStageB);
+                    const int have = w.kend - kb * BK, steps = p.dw && have < BK ? (have + 15) / 16 : 4;
+                    for (int kk = 0; kk < steps; ++kk) {
+                        const uint64_t ad = emmy::smem_desc_sw128(a_base + kk * a_step, a_lbo, 1024);
+                        const uint64_t bd = emmy::smem_desc_sw128(b_base + kk * b_step, b_lbo, 1024);
+                        if constexpr (I8) emmy::umma_i8_pair(d_tmem, ad, bd, idesc, (kb | kk) != 0 ? 1u : 0u);
+                        else emmy::umma_f16_pair(d_tmem, ad, bd, idesc, (kb | kk) != 0 ? 1u : 0u);
+                    }
+                    emmy::umma_commit_pair(emmy::smem_u32(&empty[stage]));
+                    emmy::umma_commit_pair(peer_empty + stage * 8u);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                emmy::umma_commit_pair(emmy::smem_u32(&tfull[acc]));
+                emmy::umma_commit_pair(emmy::mapa(&tfull[acc], 1));
+            }
+            // arrives on both CTAs once every pair MMA has finished
+            emmy::umma_commit_pair(emmy::smem_u32(drain));
+            emmy::umma_commit_pair(emmy::mapa(drain, 1));
+        }
+        __syncwarp();
+    } else {
+        // ---------------- output (both CTAs): own 128 channels of the tile
+        const int q = warp & 3;
+        const uint32_t leader_tempty = emmy::mapa(&tempty[0], 0);
+        uint32_t it = 0;
+        for (int64_t t = pair; t < total; t += npairs, ++it) {
+            const Tile w = tile(t);
+            const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
+            if (!emmy::mbar_wait_cluster(&tfull[acc], aphase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)) break;
+            emmy::tc_fence_after();
+            store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
+                           sStore + q * kStoreBytes, lane);
+            emmy::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) emmy::mbar_arrive_cluster(leader_tempty + acc * 8u);
+        }
+    }
+    emmy::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        // the last MMA, and the leader's last commit into this CTA, have landed (bounded)
+        if (lane == 0) {
+            volatile uint32_t never = 0u;
+            emmy::mbar_wait_cluster(drain, 0u, &never, 0u, kWaitNs);
+        }
+        __syncwarp();
+    }
+    emmy::cluster_sync();  // no CTA leaves while its peer may still signal or read it
+    if (warp == 1) {
+        emmy::tc_fence_after();
+        emmy::tmem_dealloc_pair(tmem_base, 2 * BN);
     }
 }
 

@@ -74,6 +74,10 @@ SHAPES = [
     ([40, 7, 130], 77, 101, 3),      # odd extents and strides
     ([5, 0, 64], 1, 1, 0),
     ([1100], 640, 320, 0),
+    # enough tiles for pairs of CTAs
+    ([300, 7, 300, 256, 0, 64, 257, 1000], 1536, 1032, 0),
+    ([100, 64, 1, 128, 200, 0, 65, 130], 2604, 1544, 8),
+    ([70, 1, 64, 0, 16, 63, 100, 17], 160, 2056, 0),
 ]
 
 
@@ -240,6 +244,9 @@ INT8_SHAPES = [
     ([3, 0, 50, 129], True, 272, 160, 0),
     ([300, 1, 0, 280], True, 520, 1024, 16),
     ([5, 9, 0], True, 33, 17, 1),
+    ([600], False, 4120, 640, 0),
+    ([150], False, 5120, 400, 0),
+    ([500, 0, 130, 1, 700], True, 1030, 528, 0),
 ]
 
 
