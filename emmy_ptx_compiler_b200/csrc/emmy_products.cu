@@ -38,61 +38,156 @@ static __device__ unsigned int emmy_status = 0u;
 namespace {
 
 // ---------------------------------------------------------------- row quantization
+//
+// Reads a row once: its values wait in registers while the block agrees on their largest
+// magnitude.  Bound by memory (k values read, k bytes written), as long as a value costs few
+// instructions, so nothing is converted to or from integers one by one:
+//
+// * the largest magnitude is a maximum of sign-less bit patterns, which order like the values
+//   and put infinities and NaN on top;
+// * fma(x, 1 / s, 1.5 * 2^23) rounds the exact product to an integer, ties to even, and leaves
+//   that integer in the low byte of the result's bits;
+// * 1 / s is off by half a step, so below 128 the product is off by less than 1e-5 and decides
+//   every quotient but those that close to a half.  For these the sign of x - (q +- 1/2) s, which
+//   one FMA gives exactly, tells the side.
 
-// x / s rounded to the nearest integer, exact ties to even, for the quotient of the two f32 values.
-// The product with the rounded reciprocal is off by less than 1e-4 below 128, so only a quotient
-// that close to a half is settled by the sign of x - (q +- 1/2) s, which one FMA gives exactly.
-__device__ __forceinline__ float quantize_one(float x, float s, float inv) {
-    const float t = x * inv;
-    float q = rintf(t);
-    const float d = t - q;
-    if (fabsf(d) > 0.4999f) {
+constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
+constexpr float kNearHalf = 0.4999f;
+
+// x / s to the nearest integer, exact ties to even, for the quotient of the two f32 values.
+__device__ __noinline__ int quantize_exact(float x, float s, float inv) {
+    const float q = fmaf(x, inv, kRoundMagic) - kRoundMagic;
+    const float d = fmaf(x, inv, -q);
+    float r = q;
+    if (fabsf(d) > kNearHalf) {
         const float step = d > 0.0f ? 1.0f : -1.0f;
         const float past = fmaf(-(q + 0.5f * step), s, x) * step;  // > 0: beyond the half, away from q
-        const float even = q * 0.5f;
-        if (past > 0.0f || (past == 0.0f && rintf(even) != even)) q += step;
+        if (past > 0.0f || (past == 0.0f && (static_cast<int>(q) & 1))) r = q + step;
     }
-    return fminf(fmaxf(q, -127.0f), 127.0f);
+    return static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
 }
 
-// One row for each block at a time: its largest magnitude, then its integers.
 template <typename T>
+struct Bits;
+template <>
+struct Bits<float> {
+    using U = uint32_t;
+    static constexpr uint32_t kInf = 0x7f800000u, kAbs = 0x7fffffffu;
+    static __device__ __forceinline__ float value(uint32_t u) { return __uint_as_float(u); }
+};
+template <>
+struct Bits<__nv_bfloat16> {
+    using U = uint16_t;
+    static constexpr uint32_t kInf = 0x7f80u, kAbs = 0x7fffu;
+    static __device__ __forceinline__ float value(uint32_t u) { return __uint_as_float(u << 16); }
+};
+template <>
+struct Bits<__half> {
+    using U = uint16_t;
+    static constexpr uint32_t kInf = 0x7c00u, kAbs = 0x7fffu;
+    static __device__ __forceinline__ float value(uint32_t u) {
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(u)));
+    }
+};
+
+// VEC values as they are loaded: 16 bytes, or a single value where rows are not aligned to that.
+template <typename T, int VEC>
+struct Pack {
+    using U = typename Bits<T>::U;
+    U v[VEC];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (VEC == 1) v[0] = *reinterpret_cast<const U *>(p);
+        else *reinterpret_cast<uint4 *>(v) = __ldcs(reinterpret_cast<const uint4 *>(p));
+    }
+    __device__ __forceinline__ uint32_t peak() const {
+        uint32_t m = 0;
+        if constexpr (VEC == 8) {
+            uint32_t m2 = 0;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) m2 = __vmaxu2(m2, reinterpret_cast<const uint32_t *>(v)[i] & 0x7fff7fffu);
+            m = max(m2 & 0xffffu, m2 >> 16);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) m = max(m, static_cast<uint32_t>(v[i]) & Bits<T>::kAbs);
+        }
+        return m;
+    }
+    // exact: every value goes the long way (a scale so small that its reciprocal needs lifting)
+    __device__ __forceinline__ void store(int8_t *q, float s, float inv, float lift, bool zero, bool exact) const {
+        uint32_t r[VEC];
+        float near = exact ? 1.0f : 0.0f;
+        #pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float x = Bits<T>::value(v[i]), f = fmaf(x, inv, kRoundMagic);
+            r[i] = __float_as_uint(f);
+            near = fmaxf(near, fabsf(fmaf(x, inv, kRoundMagic - f)));
+        }
+        if (near > kNearHalf) {
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) r[i] = static_cast<uint32_t>(quantize_exact(Bits<T>::value(v[i]) * lift, s, inv));
+        }
+        if constexpr (VEC == 1) {
+            *q = zero ? 0 : static_cast<int8_t>(r[0]);
+        } else {
+            uint32_t w[VEC / 4];
+            #pragma unroll
+            for (int i = 0; i < VEC / 4; ++i)
+                w[i] = zero ? 0u
+                            : __byte_perm(__byte_perm(r[4 * i], r[4 * i + 1], 0x0040),
+                                          __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x0040), 0x5410);
+            if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t *>(q) = w[0];
+        }
+    }
+};
+
+// GROUP threads for each row, PER packs of it in each thread's registers; what a longer row has
+// beyond them is read again from L2.
+template <typename T, int VEC, int GROUP, int PER>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride,
                                                             int8_t *__restrict__ q, int64_t q_stride,
                                                             float *__restrict__ scale, int64_t rows, int64_t k) {
-    __shared__ float s_peak[8];
-    __shared__ int s_bad[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const T *xr = x + r * x_stride;
-        float peak = 0.0f;
-        bool bad = false;
-        for (int64_t i = threadIdx.x; i < k; i += 256) {
-            const float v = fabsf(to_float(xr[i]));
-            bad |= !(v <= 3.402823466e38f);  // infinity or NaN
-            peak = fmaxf(peak, v);
-        }
-        for (int d = 16; d > 0; d >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, d));
-        const int any = __any_sync(0xffffffffu, bad);
+    const int tid = threadIdx.x % GROUP;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / GROUP) + threadIdx.x / GROUP;
+    const bool live = r < rows;
+    const T *xr = x + (live ? r : 0) * x_stride;
+    const int64_t packs = live ? k / VEC : 0;
+    Pack<T, VEC> held[PER];
+    uint32_t peak = 0;
+    #pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (tid + i * GROUP < packs) held[i].load(xr + (tid + i * GROUP) * static_cast<int64_t>(VEC));
+    #pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (tid + i * GROUP < packs) peak = max(peak, held[i].peak());
+    for (int64_t i = tid + PER * GROUP; i < packs; i += GROUP) {
+        Pack<T, VEC> more;
+        more.load(xr + i * VEC);
+        peak = max(peak, more.peak());
+    }
+    peak = __reduce_max_sync(0xffffffffu, peak);
+    if constexpr (GROUP > 32) {
+        __shared__ uint32_t s_peak[8];
+        if ((threadIdx.x & 31) == 0) s_peak[threadIdx.x >> 5] = peak;
         __syncthreads();
-        if (lane == 0) {
-            s_peak[warp] = peak;
-            s_bad[warp] = any;
-        }
-        __syncthreads();
-        bad = false;
-        for (int i = 0; i < 8; ++i) {
-            peak = fmaxf(peak, s_peak[i]);
-            bad |= s_bad[i] != 0;
-        }
-        const float s = __fdiv_rn(peak, 127.0f);
-        // a scale whose reciprocal could overflow is lifted, with its row, by a power of two
-        const float lift = s < 1e-30f ? 0x1p64f : 1.0f;
-        const float ls = s * lift, inv = 1.0f / ls;
-        for (int64_t i = threadIdx.x; i < k; i += 256)
-            q[r * q_stride + i] =
-                bad || s == 0.0f ? 0 : static_cast<int8_t>(quantize_one(to_float(xr[i]) * lift, ls, inv));
-        if (threadIdx.x == 0) scale[r] = bad ? __int_as_float(0x7fffffff) : s;
+        peak = __reduce_max_sync(0xffffffffu, s_peak[threadIdx.x & 7]);
+    }
+    if (!live) return;
+    const bool bad = peak >= Bits<T>::kInf;
+    const float s = __fdiv_rn(Bits<T>::value(peak), 127.0f);
+    const bool tiny = s < 1e-30f;  // lifted by a power of two, with its row, before the reciprocal
+    const float lift = tiny ? 0x1p64f : 1.0f, ls = s * lift, inv = 1.0f / ls;
+    const bool zero = bad || s == 0.0f;
+    if (tid == 0) scale[r] = bad ? __int_as_float(0x7fffffff) : s;
+    int8_t *qr = q + r * q_stride;
+    #pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (tid + i * GROUP < packs)
+            held[i].store(qr + (tid + i * GROUP) * static_cast<int64_t>(VEC), ls, inv, lift, zero, tiny);
+    for (int64_t i = tid + PER * GROUP; i < packs; i += GROUP) {
+        Pack<T, VEC> more;
+        more.load(xr + i * VEC);
+        more.store(qr + i * VEC, ls, inv, lift, zero, tiny);
     }
 }
 
@@ -234,8 +329,15 @@ int launch_pair(const Call &call, const Product &p, const Layout &lay, const CUt
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Behind the last value of an operand.
+const void *end_of(const Operand &o, int esize) {
+    if (o.inner < 1 || o.rows < 1 || o.mats < 1) return o.base;
+    const int64_t last = (o.mats - 1) * o.mat_stride + (o.rows - 1) * o.row_stride + o.inner;
+    return static_cast<const uint8_t *>(o.base) + last * esize;
+}
+
 template <bool I8>
-int launch_product(const Call &call, const Product &p, bool bf16) {
+int launch_product(const Call &call, Product p, bool bf16) {
     constexpr int esize = I8 ? 1 : 2, bk = 128 / esize;
     Layout lay{};
     lay.a_mn = p.dw || p.a_k != 1;
@@ -250,7 +352,9 @@ int launch_product(const Call &call, const Product &p, bool bf16) {
         a.mats = p.experts, a.mat_stride = p.a_e;
         b.inner = p.k, b.rows = p.rows, b.row_stride = p.b_c;
     }
-    bool tma = encode_tiled() && tma_ready(a, esize) && tma_ready(b, esize);
+    p.a_end = end_of(a, esize);
+    p.b_end = end_of(b, esize);
+    const bool tma = encode_tiled() && tma_ready(a, esize) && tma_ready(b, esize);
 
     // groups that can hold rows, and the rows of an even one
     const int64_t groups = p.experts < p.rows ? p.experts : (p.rows ? p.rows : 1);
@@ -285,7 +389,7 @@ int launch_product(const Call &call, const Product &p, bool bf16) {
         return pair == 256 ? launch_pair<I8, 256>(call, p, lay, ta, tb, pairs)
                            : launch_pair<I8, 128>(call, p, lay, ta, tb, pairs);
     }
-    const int resident = kSms * (bn <= 32 ? 2 : 1);
+    const int resident = kSms * (tma && bn <= 32 ? 2 : 1);
     int split = 1;
     while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident && kblocks >= split * 2 * 4) split *= 2;
     int64_t clusters = most(kTileM, bn);
@@ -308,6 +412,22 @@ int run_product(const char *name, int dev, int operands, const Product &p, uint6
         return report(EMMY_ERR_CUDA, "%s: device %d: %s", name, dev, cudaGetErrorString(scope.err));
     const Call call{name, dev, reinterpret_cast<cudaStream_t>(stream)};
     return operands == kS8 ? launch_product<true>(call, p, false) : launch_product<false>(call, p, operands == EMMY_BF16);
+}
+
+// A warp for each row while its registers hold the row, else the whole block.
+template <typename T>
+int launch_quantize(const Call &call, const T *x, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
+                    int64_t rows, int64_t k) {
+    constexpr int VEC = 16 / sizeof(T);
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && reinterpret_cast<uintptr_t>(q) % VEC == 0 &&
+                     x_stride % VEC == 0 && q_stride % VEC == 0 && k % VEC == 0;
+    auto go = [&](auto kernel, int group) {
+        kernel<<<static_cast<unsigned>(ceil_div(rows, 256 / group)), 256, 0, call.stream>>>(x, x_stride, q, q_stride, scale,
+                                                                                         rows, k);
+        return launched(call, cudaGetLastError());
+    };
+    if (vec) return k <= 32 * 4 * VEC ? go(quantize_rows_kernel<T, VEC, 32, 4>, 32) : go(quantize_rows_kernel<T, VEC, 256, 4>, 256);
+    return k <= 32 * 16 ? go(quantize_rows_kernel<T, 1, 32, 16>, 32) : go(quantize_rows_kernel<T, 1, 256, 16>, 256);
 }
 
 int check_common(const char *name, int dev, int64_t rows, int64_t experts, int64_t n, int64_t k) {
@@ -412,17 +532,10 @@ extern "C" int emmy_quantize_rows(int dev, int dtype, const void *x, int64_t x_s
     if (!scale || (k && (!x || !q))) return report(EMMY_ERR_INVALID, "%s: NULL pointer", name);
     DeviceScope scope(dev);
     if (scope.err != cudaSuccess) return report(EMMY_ERR_CUDA, "%s: device %d: %s", name, dev, cudaGetErrorString(scope.err));
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(rows < 148 * 8 ? rows : 148 * 8);
-    if (dtype == EMMY_BF16)
-        quantize_rows_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16 *>(x), x_stride, q, q_stride, scale, rows, k);
-    else if (dtype == EMMY_F16)
-        quantize_rows_kernel<<<grid, 256, 0, s>>>(static_cast<const __half *>(x), x_stride, q, q_stride, scale, rows, k);
-    else
-        quantize_rows_kernel<<<grid, 256, 0, s>>>(static_cast<const float *>(x), x_stride, q, q_stride, scale, rows, k);
-    const cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return report(EMMY_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
-    return EMMY_OK;
+    const Call call{name, dev, reinterpret_cast<cudaStream_t>(stream)};
+    if (dtype == EMMY_BF16) return launch_quantize(call, static_cast<const __nv_bfloat16 *>(x), x_stride, q, q_stride, scale, rows, k);
+    if (dtype == EMMY_F16) return launch_quantize(call, static_cast<const __half *>(x), x_stride, q, q_stride, scale, rows, k);
+    return launch_quantize(call, static_cast<const float *>(x), x_stride, q, q_stride, scale, rows, k);
 }
 
 extern "C" int emmy_products_status(int dev, uint32_t *status) {

@@ -17,6 +17,7 @@ constexpr int kS8 = 3;  // operand code of 8-bit products beside EMMY_F32, EMMY_
 struct Product {
     const void *a;  // A(m, k) of expert e at a[e * a_e + m * a_m + k * a_k]  (dw: k counts from the group's start)
     const void *b;  // B(c, k): forward b[(begin_e + c) * b_c + k], dw b[(begin_e + k) * b_k + c]
+    const void *a_end, *b_end;  // behind the operands' last values (plain loads stay below them)
     void *out;      // forward out[(begin_e + c) * out_c + m], dw out[e * out_e + c * out_c + m]
     const int32_t *offsets;
     const float *x_scale;  // [rows], or NULL: plain sums

@@ -141,31 +141,63 @@ __device__ __forceinline__ Tile tile_at(const Product &p, const Groups &g, int64
     return o;
 }
 
-// A panel of `rows` swizzled 128-byte rows from memory of any alignment: row r, byte b of it at
-// src + r * stride + b, zeros beyond the valid rows and values.  One warp of `warps`.
-template <typename T>
-__device__ __forceinline__ void load_panel(uint8_t *dst, const T *src, int64_t stride, int rows, int64_t rows_valid,
-                                           int64_t values_valid, int thread, int threads) {
-    constexpr int V = 16 / sizeof(T);
-    for (int i = thread; i < rows * 8; i += threads) {
-        const int r = i >> 3, j = i & 7;
-        alignas(16) T v[V];
-        const T *s = src + r * stride + j * V;
-        const int64_t have = r < rows_valid ? values_valid - j * V : 0;
-        if (have >= V && (reinterpret_cast<uintptr_t>(s) & 7) == 0) {
-            reinterpret_cast<uint2 *>(v)[0] = reinterpret_cast<const uint2 *>(s)[0];
-            reinterpret_cast<uint2 *>(v)[1] = reinterpret_cast<const uint2 *>(s)[1];
-        } else if (have >= V && (reinterpret_cast<uintptr_t>(s) & 3) == 0) {
-            #pragma unroll
-            for (int b = 0; b < 4; ++b) reinterpret_cast<uint32_t *>(v)[b] = reinterpret_cast<const uint32_t *>(s)[b];
-        } else {
-            #pragma unroll
-            for (int b = 0; b < V; ++b) {
-                if (b < have) v[b] = s[b];
-                else v[b] = T(0);
-            }
+// Operands that TMA cannot address (rows that start off a 16-byte boundary) are loaded in units of
+// 64 bytes of a row, as the five aligned 16-byte words that cover them; the bytes are shifted into
+// place in registers.  A word is read whole where it lies inside the operand, whichever of its
+// bytes are wanted; at the operand's two ends it is put together from its bytes.
+struct Unit {
+    uint4 w[5];
+};
+
+__device__ __noinline__ uint4 load_edge_word(const uint8_t *at, const uint8_t *lo, const uint8_t *hi) {
+    alignas(16) uint8_t v[16];
+    for (int i = 0; i < 16; ++i) v[i] = at + i >= lo && at + i < hi ? at[i] : 0;
+    return *reinterpret_cast<const uint4 *>(v);
+}
+
+// `bytes` (at most 64, may be negative) of the unit at `src` are wanted.
+__device__ __forceinline__ void load_unit(Unit &u, const uint8_t *src, int64_t bytes, const uint8_t *lo,
+                                          const uint8_t *hi) {
+    const uint8_t *at = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(src) & ~uintptr_t(15));
+    const uint8_t *end = src + (bytes < 64 ? bytes : 64);
+    #pragma unroll
+    for (int i = 0; i < 5; ++i, at += 16) {
+        u.w[i] = make_uint4(0, 0, 0, 0);
+        if (bytes > 0 && at < end) {
+            if (at >= lo && at + 16 <= hi) u.w[i] = *reinterpret_cast<const uint4 *>(at);
+            else u.w[i] = load_edge_word(at, lo, hi);
         }
-        *reinterpret_cast<uint4 *>(dst + r * kBlockBytes + ((j ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4 *>(v);
+    }
+}
+
+// The first `keep` bytes of a word (any value; below 0 counts as 0).
+__device__ __forceinline__ uint32_t keep_bytes(uint32_t v, int64_t keep) {
+    return keep >= 4 ? v : keep <= 0 ? 0u : v & ((1u << (8 * static_cast<int>(keep))) - 1u);
+}
+
+// Shift a unit into place and store its four 16-byte chunks, zeros behind `bytes`, into row `row` of a
+// swizzled panel; `half`: which 64 bytes of the 128-byte row.
+__device__ __forceinline__ void store_unit(const Unit &u, const uint8_t *src, int64_t bytes, uint8_t *panel, int row,
+                                           int half) {
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src)) & 15u, bits = (off & 3u) * 8u;
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&u);
+    uint32_t v[17];
+    #pragma unroll
+    for (int i = 0; i < 17; ++i) {
+        // word off / 4 + i of the 20, without indexing registers by a variable
+        const uint32_t near = off & 4u ? w[i + 1] : w[i], far = off & 4u ? w[i + 3] : w[i + 2];
+        v[i] = off & 8u ? far : near;
+    }
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t c[4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            c[i] = __funnelshift_r(v[4 * j + i], v[4 * j + i + 1], bits);
+            if (bytes < 64) c[i] = keep_bytes(c[i], bytes - 16 * j - 4 * i);
+        }
+        *reinterpret_cast<uint4 *>(panel + row * kBlockBytes + (((half * 4 + j) ^ (row & 7)) << 4)) =
+            make_uint4(c[0], c[1], c[2], c[3]);
     }
 }
 
@@ -298,12 +330,13 @@ struct TcConfig {
     static constexpr uint32_t kStage = kStageA + kStageB;
     static constexpr uint32_t kRed = BN * kTileM * 4;  // partial sums for the cluster
     static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
-    static constexpr int kThreads = TMA ? 192 : 320;
+    static constexpr int kLoaders = TMA ? 1 : 8;  // warps that fill the stages
+    static constexpr int kThreads = TMA ? 192 : 192 + 32 * kLoaders;
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + 256;
     static constexpr uint32_t kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
-// Warp 0 loads operand tiles by TMA (TMA false: warps 6 to 9 do, with plain loads, for addresses
+// Warp 0 loads operand tiles by TMA (TMA false: warps 6 to 13 do, with plain loads, for rows
 // TMA cannot take), warp 1 issues the MMAs into one of two accumulators, warps 2 to 5 turn the
 // other into output.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
 // added in rank order through distributed shared memory, each CTA finishing its share of columns:
@@ -316,7 +349,6 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
     using T = std::conditional_t<I8, int8_t, uint16_t>;
     constexpr int STAGES = Cfg::kStages;
     constexpr int BK = I8 ? 128 : 64;
-    constexpr uint32_t LOADERS = TMA ? 1 : 4;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ Groups g;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -335,7 +367,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
 
     if (threadIdx.x == 64) {
         for (int s = 0; s < STAGES; ++s) {
-            emmy::mbar_init(&full[s], LOADERS);
+            emmy::mbar_init(&full[s], Cfg::kLoaders);
             emmy::mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -409,32 +441,55 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
             }
             __syncwarp();
         } else if (!TMA && warp >= 6) {
-            const int th = threadIdx.x - 192;
+            // 256 threads: one unit of A (128 rows x 2 halves) and at most one of B each, the next
+            // block's loads in flight while this block's are stored
+            const int th = threadIdx.x - 192, half = th & 1;
+            const uint8_t *a_lo = static_cast<const uint8_t *>(p.a), *a_hi = static_cast<const uint8_t *>(p.a_end);
+            const uint8_t *b_lo = static_cast<const uint8_t *>(p.b), *b_hi = static_cast<const uint8_t *>(p.b_end);
+            const bool has_b = th < 2 * BN;
             for (int64_t t = first; t < last && ok; t += step) {
                 const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
                 const T *ae = static_cast<const T *>(p.a) + (p.dw ? w.begin * p.a_k : w.e * p.a_e);
                 const T *be = static_cast<const T *>(p.b) + w.begin * (p.dw ? p.b_k : p.b_c);
+                Unit ua, ub;
+                const uint8_t *pa = nullptr, *pb = nullptr;
+                int64_t na = 0, nb = 0;
+                // where this thread's units of block kb lie, and how many of their bytes are wanted
+                auto load = [&](int kb) {
+                    const int64_t k0 = static_cast<int64_t>(kb) * BK, kleft = w.kend - k0;
+                    const int64_t row = th >> 1, krow = row & 63, panel = row >> 6;
+                    if (lay.a_mn) {
+                        const int64_t m = w.m0 + 64 * panel;
+                        pa = reinterpret_cast<const uint8_t *>(ae + (k0 + krow) * p.a_k + m);
+                        na = krow < kleft ? (p.m - m) * static_cast<int64_t>(sizeof(T)) : 0;
+                    } else {
+                        pa = reinterpret_cast<const uint8_t *>(ae + (w.m0 + row) * p.a_m + k0);
+                        na = row < p.m - w.m0 ? kleft * static_cast<int64_t>(sizeof(T)) : 0;
+                    }
+                    pa += 64 * half;
+                    na -= 64 * half;
+                    load_unit(ua, pa, na, a_lo, a_hi);
+                    if (!has_b) return;
+                    if (lay.b_mn) {
+                        pb = reinterpret_cast<const uint8_t *>(be + (k0 + krow) * p.b_k + w.c0 + 64 * panel);
+                        nb = krow < kleft ? (w.cols - 64 * panel) * static_cast<int64_t>(sizeof(T)) : 0;
+                    } else {
+                        pb = reinterpret_cast<const uint8_t *>(be + (w.c0 + row) * p.b_c + k0);
+                        nb = row < w.cols ? kleft * static_cast<int64_t>(sizeof(T)) : 0;
+                    }
+                    pb += 64 * half;
+                    nb -= 64 * half;
+                    load_unit(ub, pb, nb, b_lo, b_hi);
+                };
+                if (w.kb0 < w.kb1) load(w.kb0);
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
                     if (!emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
                         ok = false;
                         break;
                     }
-                    uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
-                    const int64_t k0 = static_cast<int64_t>(kb) * BK;
-                    if (lay.a_mn) {
-                        for (int j = 0; j < 2; ++j)
-                            load_panel(a + j * kPanel, ae + k0 * p.a_k + w.m0 + 64 * j, p.a_k, 64, w.kend - k0,
-                                       p.m - w.m0 - 64 * j, th, 128);
-                    } else {
-                        load_panel(a, ae + w.m0 * p.a_m + k0, p.a_m, kTileM, p.m - w.m0, w.kend - k0, th, 128);
-                    }
-                    if (lay.b_mn) {
-                        for (int j = 0; j < BN / 64; ++j)
-                            load_panel(b + j * kPanel, be + k0 * p.b_k + w.c0 + 64 * j, p.b_k, 64, w.kend - k0,
-                                       w.cols - 64 * j, th, 128);
-                    } else {
-                        load_panel(b, be + w.c0 * p.b_c + k0, p.b_c, BN, w.cols, w.kend - k0, th, 128);
-                    }
+                    // a 128-row K-major tile and two 64-row panels are laid out alike
+                    store_unit(ua, pa, na, sA + stage * kStageA, th >> 1, half);
+                    if (has_b) store_unit(ub, pb, nb, sB + stage * Cfg::kStageB, th >> 1, half);
                     emmy::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) emmy::mbar_arrive(&full[stage]);
@@ -442,6 +497,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                         stage = 0;
                         phase ^= 1u;
                     }
+                    if (kb + 1 < w.kb1) load(kb + 1);
                 }
             }
         } else if (warp == 1) {
