@@ -150,6 +150,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T *__restrict_
     const int tid = threadIdx.x % GROUP;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / GROUP) + threadIdx.x / GROUP;
     const bool live = r < rows;
+    emmy::wait_for_prior_grid();
+    emmy::let_next_grid_start();
     const T *xr = x + (live ? r : 0) * x_stride;
     const int64_t packs = live ? k / VEC : 0;
     Pack<T, VEC> held[PER];
@@ -284,6 +286,24 @@ int launched(const Call &call, cudaError_t err) {
     return report(EMMY_ERR_CUDA, "%s: launch: %s", call.name, cudaGetErrorString(err));
 }
 
+cudaLaunchConfig_t config(const Call &call, int64_t blocks, int threads, uint32_t smem) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = call.stream;
+    return cfg;
+}
+
+// The kernel may be set up while the one before it on the stream still runs.  Every kernel here
+// waits for that one's end before it touches a buffer, so the order on the stream holds.
+cudaLaunchAttribute early_start() {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    return attr;
+}
+
 using TcKernel = void (*)(Product, Layout, CUtensorMap, CUtensorMap);
 
 // A launch of clusters of `cluster` CTAs.  `ready` marks the devices on which the kernel's
@@ -297,16 +317,12 @@ int launch_clusters(const Call &call, TcKernel kernel, std::atomic<uint64_t> &re
         if (err != cudaSuccess) return launched(call, err);
         ready.fetch_or(1ull << call.dev, std::memory_order_release);
     }
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
-    cfg.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = call.stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchConfig_t cfg = config(call, clusters * cluster, threads, smem);
+    cudaLaunchAttribute attrs[2] = {early_start(), {}};
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
     return launched(call, cudaLaunchKernelEx(&cfg, kernel, p, lay, ta, tb));
 }
 
@@ -323,8 +339,8 @@ template <bool I8, int BN>
 int launch_pair(const Call &call, const Product &p, const Layout &lay, const CUtensorMap &ta, const CUtensorMap &tb,
                 int64_t pairs) {
     static std::atomic<uint64_t> ready{0};
-    return launch_clusters(call, product_pair_kernel<I8, BN>, ready, p, lay, ta, tb, pairs, 2, 192,
-                           PairConfig<BN>::kSmem);
+    return launch_clusters(call, product_pair_kernel<I8, BN>, ready, p, lay, ta, tb, pairs, 2,
+                           PairConfig<BN>::kThreads, PairConfig<BN>::kSmem);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -372,6 +388,8 @@ int launch_product(const Call &call, Product p, bool bf16) {
         if (cext > 192 && tiles(256, 256) >= kSms / 4) pair = 256;
         else if (tiles(256, 128) >= kSms / 4) pair = 128;
     }
+    if (most(kTileM, p.dw ? 64 : 16) > kMaxExtent)
+        return report(EMMY_ERR_INVALID, "%s: an output of more than 2^31 tiles is not supported", call.name);
     const int bn = pair ? pair : p.dw ? 128 : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
 
     CUtensorMap ta{}, tb{};
@@ -422,9 +440,11 @@ int launch_quantize(const Call &call, const T *x, int64_t x_stride, int8_t *q, i
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && reinterpret_cast<uintptr_t>(q) % VEC == 0 &&
                      x_stride % VEC == 0 && q_stride % VEC == 0 && k % VEC == 0;
     auto go = [&](auto kernel, int group) {
-        kernel<<<static_cast<unsigned>(ceil_div(rows, 256 / group)), 256, 0, call.stream>>>(x, x_stride, q, q_stride, scale,
-                                                                                         rows, k);
-        return launched(call, cudaGetLastError());
+        cudaLaunchConfig_t cfg = config(call, ceil_div(rows, 256 / group), 256, 0);
+        cudaLaunchAttribute attr = early_start();
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        return launched(call, cudaLaunchKernelEx(&cfg, kernel, x, x_stride, q, q_stride, scale, rows, k));
     };
     if (vec) return k <= 32 * 4 * VEC ? go(quantize_rows_kernel<T, VEC, 32, 4>, 32) : go(quantize_rows_kernel<T, VEC, 256, 4>, 256);
     return k <= 32 * 16 ? go(quantize_rows_kernel<T, 1, 32, 16>, 32) : go(quantize_rows_kernel<T, 1, 256, 16>, 256);

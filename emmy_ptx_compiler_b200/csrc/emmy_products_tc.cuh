@@ -86,6 +86,11 @@ __device__ __forceinline__ void fence_proxy_async() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// Programmatic launches: a kernel may start while the one before it on the stream still runs; it
+// waits here, before its first access to memory that others write, until that one has finished.
+__device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
@@ -118,26 +123,36 @@ struct Layout {
 };
 
 struct Tile {
-    int e, begin, cols, kend, kb0, kb1;
-    int64_t m0, c0;
+    int e, begin;   // expert and its first row
+    int m0, c0;     // first channel, first output row (of the group; dw: of the matrix)
+    int cols;       // output rows in the tile
+    int kend;       // extent of the sum
+    int kb0, kb1;   // blocks of it that this CTA sums
 };
 
-// Tile t of the launch, and the k blocks [kb0, kb1) that this CTA of the cluster sums.
-__device__ __forceinline__ Tile tile_at(const Product &p, const Groups &g, int64_t t, int64_t mt, int &e, int col_tile,
+// Channel tiles that go over all rows of their expert together: what they read of the rows stays
+// in L2 from one to the next.
+constexpr int kSweep = 8;
+
+// Tile t of the launch (tm x col_tile; host code keeps the tiles within 31 bits).  `e` is a cursor:
+// tiles of one caller come in ascending order.  A cluster of `split` CTAs divides the sum.
+__device__ __forceinline__ Tile tile_at(const Product &p, const Groups &g, int t, int mt, int &e, int tm, int col_tile,
                                         int bk, uint32_t rank, uint32_t split) {
     while (t >= mt * g.tiles[e + 1]) ++e;
-    const int64_t r = t - mt * g.tiles[e];
     const int begin = g.row[e], count = g.row[e + 1] - begin;
+    const uint32_t r = t - mt * g.tiles[e], sweep_tiles = kSweep * (g.tiles[e + 1] - g.tiles[e]);
+    const uint32_t sweep = r / sweep_tiles, in = r - sweep * sweep_tiles, first = sweep * kSweep;
+    const uint32_t wide = min(static_cast<uint32_t>(kSweep), mt - first), ci = in / wide;
     Tile o;
     o.e = e;
     o.begin = begin;
-    o.m0 = r % mt * kTileM;
-    o.c0 = r / mt * col_tile;
-    o.cols = static_cast<int>(min(static_cast<int64_t>(col_tile), (p.dw ? p.c : count) - o.c0));
+    o.m0 = static_cast<int>(first + in - ci * wide) * tm;
+    o.c0 = static_cast<int>(ci) * col_tile;
+    o.cols = min(col_tile, (p.dw ? static_cast<int>(p.c) : count) - o.c0);
     o.kend = p.dw ? count : static_cast<int>(p.k);
-    const int nkb = o.kend / bk + (o.kend % bk != 0);
-    o.kb0 = static_cast<int>(static_cast<int64_t>(nkb) * rank / split);
-    o.kb1 = static_cast<int>(static_cast<int64_t>(nkb) * (rank + 1) / split);
+    const uint32_t nkb = o.kend / bk + (o.kend % bk != 0);
+    o.kb0 = static_cast<int>(nkb * rank / split);
+    o.kb1 = static_cast<int>(nkb * (rank + 1) / split);
     return o;
 }
 
@@ -212,14 +227,27 @@ __device__ __forceinline__ float sum_value(uint32_t bits) {
     else return __uint_as_float(bits);
 }
 
-// Scale and store one finished sum: column c of the tile, channel m.
+// Where channel m of output row c of the tile goes.
+__device__ __forceinline__ int64_t out_index(const Product &p, const Tile &t, int64_t m, int c) {
+    return (p.dw ? t.e * p.out_e : t.begin * p.out_c) + (t.c0 + static_cast<int64_t>(c)) * p.out_c + m;
+}
+
+// Scale of a channel, and its bias.
+struct Channel {
+    float scale = 0.0f, bias = 0.0f;
+};
+__device__ __forceinline__ Channel channel(const Product &p, const Tile &t, int64_t m) {
+    Channel c;
+    if (m < p.m) {
+        c.scale = p.w_scale[t.e * p.m + m];
+        if (p.bias) c.bias = p.bias[t.e * p.m + m];
+    }
+    return c;
+}
 template <bool I8>
-__device__ __forceinline__ void finish(const Product &p, const Tile &t, int64_t m, int col, uint32_t bits, float w_scale,
-                                       float bias) {
-    float v = sum_value<I8>(bits);
-    const int64_t c = t.c0 + col;
-    if constexpr (I8) v = v * p.x_scale[t.begin + c] * w_scale + bias;
-    store_out(p.out, p.out_type, (p.dw ? t.e * p.out_e : t.begin * p.out_c) + c * p.out_c + m, v);
+__device__ __forceinline__ float scaled(uint32_t bits, float row_scale, const Channel &c) {
+    if constexpr (I8) return sum_value<true>(bits) * row_scale * c.scale + c.bias;
+    else return sum_value<false>(bits);
 }
 
 // Staging of a warp's 32 channels x 32 output rows: 64 bytes a row, 80 apart, so that neither the
@@ -235,72 +263,76 @@ __device__ __forceinline__ uint32_t pack16(bool bf16, float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// The accumulator's channels lie on lanes, the output's along a row.  16-bit outputs are transposed
-// on the way: fragments of 8 x 8 go to shared memory through stmatrix, and 4 lanes then write each
-// 64-byte piece of an output row 16 bytes at a time (8 stores a block instead of 32, and the
-// conversion packs two values).  f32 outputs need no help: 32 lanes write 128 bytes of a row.
+// Output rows [from, to) of a warp's 32 channels, from the accumulator at `taddr`.  Its channels lie
+// on lanes, the output's along a row.  16-bit outputs are transposed on the way: fragments of 8 x 8
+// go to shared memory through stmatrix, and 4 lanes then write each 64-byte piece of an output row
+// 16 bytes at a time (4 stores for 32 rows instead of 32, and the conversion packs two values).  f32
+// outputs need no help: 32 lanes write 128 bytes of a row.  `empty`: the sum had no terms.
 template <bool I8>
-__device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int64_t mq, uint32_t taddr, bool empty,
-                                           uint8_t *buf, int lane) {
+__device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int mq, uint32_t taddr, bool empty, int from,
+                                           int to, uint8_t *buf, int lane) {
+    if (to > w.cols) to = w.cols;
+    if (from >= to) return;
     if (p.out_type == EMMY_F32) {
         const int64_t m = mq + lane;
-        float ws = 0.0f, bias = 0.0f;
-        if (I8 && m < p.m) {
-            ws = p.w_scale[w.e * p.m + m];
-            if (p.bias) bias = p.bias[w.e * p.m + m];
-        }
+        Channel ch;
+        if constexpr (I8) ch = channel(p, w, m);
+        float *out = static_cast<float *>(p.out) + out_index(p, w, m, from);
         #pragma unroll 1
-        for (int c = 0; c < w.cols; c += 16) {
-            uint32_t r[16];
-            emmy::tmem_ld_32x32b_x16(taddr + c, r);
+        for (int c = from; c < to; c += 32, out += 32 * p.out_c) {
+            uint32_t r[32];
+            emmy::tmem_ld_32x32b_x32(taddr + c, r);
+            float xs = 0.0f;
+            if (I8 && c + lane < to) xs = p.x_scale[w.begin + w.c0 + c + lane];
             emmy::tmem_ld_wait();
-            if (m < p.m) {
+            if (empty) {
                 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (c + j < w.cols) finish<I8>(p, w, m, c + j, empty ? 0u : r[j], ws, bias);
+                for (int j = 0; j < 32; ++j) r[j] = 0u;
+            }
+            float *o = out;
+            #pragma unroll
+            for (int j = 0; j < 32; ++j, o += p.out_c) {
+                const float v = scaled<I8>(r[j], I8 ? __shfl_sync(0xffffffffu, xs, j) : 0.0f, ch);
+                if (m < p.m && c + j < to) *o = v;
             }
         }
         return;
     }
-    uint16_t *out = static_cast<uint16_t *>(p.out) +
-                    ((p.dw ? w.e * p.out_e : w.begin * p.out_c) + w.c0 * p.out_c + mq);
+    const int piece = lane & 3;
+    uint16_t *out = static_cast<uint16_t *>(p.out) + out_index(p, w, mq, from);
     const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && ((p.out_c | p.out_e | p.m) & 7) == 0;
-    const bool bf16 = p.out_type == EMMY_BF16;
-    float ws[4] = {}, bias[4] = {};
+    const bool bf16 = p.out_type == EMMY_BF16, piece_in = mq + piece * 8 < p.m;
+    Channel ch[4];
     if constexpr (I8) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t m = mq + lane / 4 + 8 * i;
-            if (m < p.m) {
-                ws[i] = p.w_scale[w.e * p.m + m];
-                if (p.bias) bias[i] = p.bias[w.e * p.m + m];
-            }
-        }
+        for (int i = 0; i < 4; ++i) ch[i] = channel(p, w, mq + lane / 4 + 8 * i);
     }
     #pragma unroll 1
-    for (int c = 0; c < w.cols; c += 32) {
+    for (int c = from; c < to; c += 32, out += 32 * p.out_c) {
+        uint32_t r[2][16];
+        emmy::tmem_ld_16x256b_x4(taddr + c, r[0]);
+        emmy::tmem_ld_16x256b_x4(taddr + (16u << 16) + c, r[1]);
         float xs[8];
         if constexpr (I8) {
             #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int col = c + 8 * (i >> 1) + 2 * (lane & 3) + (i & 1);
-                xs[i] = col < w.cols ? p.x_scale[w.begin + w.c0 + col] : 0.0f;
+                const int col = c + 8 * (i >> 1) + 2 * piece + (i & 1);
+                xs[i] = col < to ? p.x_scale[w.begin + w.c0 + col] : 0.0f;
             }
+        }
+        emmy::tmem_ld_wait();
+        if (empty) {
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) r[0][i] = r[1][i] = 0u;
         }
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t r[16], v[8];
-            emmy::tmem_ld_16x256b_x4(taddr + (static_cast<uint32_t>(16 * h) << 16) + c, r);
-            emmy::tmem_ld_wait();
+            uint32_t v[8];
             #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float lo = sum_value<I8>(empty ? 0u : r[2 * i]), hi = sum_value<I8>(empty ? 0u : r[2 * i + 1]);
-                if constexpr (I8) {
-                    const int row = 2 * h + (i & 1);
-                    lo = lo * xs[i >> 1 << 1] * ws[row] + bias[row];
-                    hi = hi * xs[(i >> 1 << 1) + 1] * ws[row] + bias[row];
-                }
-                v[i] = pack16(bf16, lo, hi);
+                const int row = 2 * h + (i & 1), col = i >> 1 << 1;
+                v[i] = pack16(bf16, scaled<I8>(r[h][2 * i], I8 ? xs[col] : 0.0f, ch[row]),
+                              scaled<I8>(r[h][2 * i + 1], I8 ? xs[col + 1] : 0.0f, ch[row]));
             }
             const uint32_t at = emmy::smem_u32(buf) + ((lane >> 4) * 8 + (lane & 7)) * kStoreRow +
                                 (16 * h + 8 * ((lane >> 3) & 1)) * 2;
@@ -311,14 +343,14 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int6
         if (vec) {
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = i * 8 + (lane >> 2), piece = lane & 3;
-                if (c + row < w.cols && mq + piece * 8 < p.m)
-                    *reinterpret_cast<uint4 *>(out + (c + row) * p.out_c + piece * 8) =
+                const int row = i * 8 + (lane >> 2);
+                if (piece_in && c + row < to)
+                    *reinterpret_cast<uint4 *>(out + row * p.out_c + piece * 8) =
                         *reinterpret_cast<const uint4 *>(buf + row * kStoreRow + piece * 16);
             }
         } else if (mq + lane < p.m) {
-            for (int row = 0; row < 32 && c + row < w.cols; ++row)
-                out[(c + row) * p.out_c + lane] = *reinterpret_cast<const uint16_t *>(buf + row * kStoreRow + lane * 2);
+            for (int row = 0; row < 32 && c + row < to; ++row)
+                out[row * p.out_c + lane] = *reinterpret_cast<const uint16_t *>(buf + row * kStoreRow + lane * 2);
         }
         __syncwarp();
     }
@@ -330,15 +362,16 @@ struct TcConfig {
     static constexpr uint32_t kStage = kStageA + kStageB;
     static constexpr uint32_t kRed = BN * kTileM * 4;  // partial sums for the cluster
     static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
-    static constexpr int kLoaders = TMA ? 1 : 8;  // warps that fill the stages
-    static constexpr int kThreads = TMA ? 192 : 192 + 32 * kLoaders;
+    static constexpr int kOut = BN >= 64 ? 8 : 4;  // warps that turn sums into output
+    static constexpr int kLoaders = TMA ? 1 : 8;   // warps that fill the stages
+    static constexpr int kThreads = 64 + 32 * kOut + (TMA ? 0 : 32 * kLoaders);
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + 256;
     static constexpr uint32_t kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
-// Warp 0 loads operand tiles by TMA (TMA false: warps 6 to 13 do, with plain loads, for rows
-// TMA cannot take), warp 1 issues the MMAs into one of two accumulators, warps 2 to 5 turn the
-// other into output.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
+// Warp 0 loads operand tiles by TMA (TMA false: the last 8 warps do, with plain loads, for
+// rows TMA cannot take), warp 1 issues the MMAs into one of two accumulators, the warps from 2 on
+// turn the other into output, 4 or 8 of them: a warp reaches 32 of the 128 lanes.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
 // added in rank order through distributed shared memory, each CTA finishing its share of columns:
 // the result depends on neither timing nor the number of SMs.
 template <bool I8, int BN, bool TMA>
@@ -372,7 +405,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             emmy::mbar_init(&tfull[a], 1);
-            emmy::mbar_init(&tempty[a], 4);
+            emmy::mbar_init(&tempty[a], Cfg::kOut);
         }
         emmy::mbar_init(drain, 1);
         *abort_flag = 0u;
@@ -387,28 +420,30 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
             emmy::tma_prefetch(&tm_a);
             emmy::tma_prefetch(&tm_b);
         }
-        load_groups(g, p, BN);
     }
+    emmy::wait_for_prior_grid();
+    if (warp == 0) load_groups(g, p, BN);
     emmy::tc_fence_before();
     __syncthreads();
     emmy::tc_fence_after();
+    emmy::let_next_grid_start();
     const uint32_t tmem_base = *tmem_holder;
 
-    const int64_t mt = (p.m + kTileM - 1) / kTileM, total = mt * g.tiles[p.experts];
-    const int64_t step = gridDim.x / split;
+    const int mt = static_cast<int>((p.m + kTileM - 1) / kTileM), total = mt * g.tiles[p.experts];
+    const int step = static_cast<int>(gridDim.x / split);
     uint32_t stage = 0, phase = 0, it = 0;
     uint32_t issued = 0u, parity_bits = 0u;  // producer: loads in flight for each stage and their parity
     bool ok = true;
     int e = 0;
     // Without a cluster each role runs through all of the CTA's tiles at its own pace; a cluster
     // takes one tile at a time, because its CTAs meet after each.
-    for (int64_t first = blockIdx.x / split; first < total; first += split > 1 ? step : total) {
-        const int64_t last = split > 1 ? first + 1 : total;
+    for (int first = static_cast<int>(blockIdx.x / split); first < total; first += split > 1 ? step : total) {
+        const int last = split > 1 ? first + 1 : total;
         if (TMA && warp == 0) {
             if (lane == 0) {
-                for (int64_t t = first; t < last && ok; t += step) {
-                    const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
-                    const int m0 = static_cast<int>(w.m0), c0 = static_cast<int>(w.c0);
+                for (int t = first; t < last && ok; t += step) {
+                    const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
+                    const int m0 = w.m0, c0 = w.c0;
                     for (int kb = w.kb0; kb < w.kb1; ++kb) {
                         if (!emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
                             ok = false;
@@ -440,15 +475,15 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                 }
             }
             __syncwarp();
-        } else if (!TMA && warp >= 6) {
+        } else if (!TMA && warp >= 2 + Cfg::kOut) {
             // 256 threads: one unit of A (128 rows x 2 halves) and at most one of B each, the next
             // block's loads in flight while this block's are stored
-            const int th = threadIdx.x - 192, half = th & 1;
+            const int th = threadIdx.x - 64 - 32 * Cfg::kOut, half = th & 1;
             const uint8_t *a_lo = static_cast<const uint8_t *>(p.a), *a_hi = static_cast<const uint8_t *>(p.a_end);
             const uint8_t *b_lo = static_cast<const uint8_t *>(p.b), *b_hi = static_cast<const uint8_t *>(p.b_end);
             const bool has_b = th < 2 * BN;
-            for (int64_t t = first; t < last && ok; t += step) {
-                const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
+            for (int t = first; t < last && ok; t += step) {
+                const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const T *ae = static_cast<const T *>(p.a) + (p.dw ? w.begin * p.a_k : w.e * p.a_e);
                 const T *be = static_cast<const T *>(p.b) + w.begin * (p.dw ? p.b_k : p.b_c);
                 Unit ua, ub;
@@ -506,8 +541,8 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
             // one MMA takes 32 bytes of k: along a swizzled row when k is contiguous, else 16 rows further
             const uint32_t a_step = lay.a_mn ? 16 * kBlockBytes : 32, a_lbo = lay.a_mn ? kPanel : 16;
             const uint32_t b_step = lay.b_mn ? 16 * kBlockBytes : 32, b_lbo = lay.b_mn ? kPanel : 16;
-            for (int64_t t = first; t < last && ok; t += step, ++it) {
-                const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
+            for (int t = first; t < last && ok; t += step, ++it) {
+                const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
                 if (!emmy::mbar_wait(&tempty[acc], aphase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) {
                     ok = false;
@@ -556,42 +591,43 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                 if (lane == 0) emmy::umma_commit(&tfull[acc]);
                 __syncwarp();
             }
-        } else if (warp >= 2 && warp < 6) {
-            const int q = warp & 3;
-            for (int64_t t = first; t < last && ok; t += step, ++it) {
-                const Tile w = tile_at(p, g, t, mt, e, BN, BK, rank, split);
+        } else if (warp >= 2 && warp < 2 + Cfg::kOut) {
+            const int q = warp & 3, part = (warp - 2) >> 2;
+            constexpr int PARTS = Cfg::kOut / 4, SPAN = BN / PARTS;
+            for (int t = first; t < last && ok; t += step, ++it) {
+                const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
                 if (!emmy::mbar_wait(&tfull[acc], aphase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)) {
                     ok = false;
                     break;
                 }
                 emmy::tc_fence_after();
-                const int64_t m = w.m0 + q * 32 + lane;
-                float w_scale = 0.0f, bias = 0.0f;
+                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+                const bool none = w.kb0 == w.kb1;  // nothing was accumulated
                 if (BN >= 64 && split == 1) {
                     // the sums' exchange buffer is free without a cluster
-                    store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN,
-                                   w.kb0 == w.kb1, reinterpret_cast<uint8_t *>(red) + q * kStoreBytes, lane);
-                    emmy::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) emmy::mbar_arrive(&tempty[acc]);
-                    continue;
-                }
-                if (I8 && split == 1 && m < p.m) {
-                    w_scale = p.w_scale[w.e * p.m + m];
-                    if (p.bias) bias = p.bias[w.e * p.m + m];
-                }
-                #pragma unroll 1
-                for (int c = 0; c < w.cols; c += 16) {
-                    uint32_t r[16];
-                    emmy::tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN + c, r);
-                    emmy::tmem_ld_wait();
-                    #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (c + j >= w.cols) break;
-                        const uint32_t v = w.kb0 < w.kb1 ? r[j] : 0u;  // no k: nothing was accumulated
-                        if (split > 1) red[(c + j) * kTileM + q * 32 + lane] = v;
-                        else if (m < p.m) finish<I8>(p, w, m, c + j, v, w_scale, bias);
+                    store_tile<I8>(p, w, w.m0 + q * 32, taddr, none, part * SPAN, (part + 1) * SPAN,
+                                   reinterpret_cast<uint8_t *>(red) + (warp - 2) * kStoreBytes, lane);
+                } else {
+                    // few columns, or parts of sums: channels of a column are neighbours either way
+                    const int64_t m = w.m0 + q * 32 + lane;
+                    Channel ch;
+                    if (I8 && split == 1) ch = channel(p, w, m);
+                    #pragma unroll 1
+                    for (int c = part * SPAN; c < min((part + 1) * SPAN, w.cols); c += 16) {
+                        uint32_t r[16];
+                        emmy::tmem_ld_32x32b_x16(taddr + c, r);
+                        emmy::tmem_ld_wait();
+                        #pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            if (c + j >= w.cols) break;
+                            const uint32_t v = none ? 0u : r[j];
+                            if (split > 1)
+                                red[(c + j) * kTileM + q * 32 + lane] = v;
+                            else if (m < p.m)
+                                store_out(p.out, p.out_type, out_index(p, w, m, c + j),
+                                          scaled<I8>(v, I8 ? p.x_scale[w.begin + w.c0 + c + j] : 0.0f, ch));
+                        }
                     }
                 }
                 emmy::tc_fence_before();
@@ -602,23 +638,21 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
         if (split > 1) {
             __syncwarp();
             emmy::cluster_sync();  // every CTA's partial sums are in its shared memory
-            if (warp >= 2 && warp < 6 && ok) {
-                const Tile w = tile_at(p, g, first, mt, e, BN, BK, rank, split);
-                const int lm = (warp & 3) * 32 + lane;
+            if (warp >= 2 && warp < 2 + Cfg::kOut && ok) {
+                const Tile w = tile_at(p, g, first, mt, e, kTileM, BN, BK, rank, split);
+                const int lm = (warp & 3) * 32 + lane, part = (warp - 2) >> 2, parts = Cfg::kOut / 4;
                 const int64_t m = w.m0 + lm;
                 if (m < p.m) {
-                    float w_scale = 0.0f, bias = 0.0f;
-                    if (I8) {
-                        w_scale = p.w_scale[w.e * p.m + m];
-                        if (p.bias) bias = p.bias[w.e * p.m + m];
-                    }
-                    for (int c = rank; c < w.cols; c += split) {
+                    Channel ch;
+                    if constexpr (I8) ch = channel(p, w, m);
+                    for (int c = rank + split * part; c < w.cols; c += split * parts) {
                         uint32_t sum = 0u;  // 0 of either type
                         for (uint32_t s = 0; s < split; ++s) {
                             const uint32_t v = emmy::ld_cluster_u32(emmy::mapa(&red[c * kTileM + lm], s));
                             sum = I8 ? sum + v : __float_as_uint(__uint_as_float(sum) + __uint_as_float(v));
                         }
-                        finish<I8>(p, w, m, c, sum, w_scale, bias);
+                        store_out(p.out, p.out_type, out_index(p, w, m, c),
+                                  scaled<I8>(sum, I8 ? p.x_scale[w.begin + w.c0 + c] : 0.0f, ch));
                     }
                 }
             }
@@ -660,12 +694,13 @@ struct PairConfig {
     static constexpr uint32_t kStageB = BN / 2 * kBlockBytes;
     static constexpr uint32_t kStage = kStageA + kStageB;
     static constexpr int kStages = BN == 256 ? 6 : 8;
-    static constexpr uint32_t kSmem = 1024 + kStages * kStage + 4 * kStoreBytes + 256;
-    static constexpr int kSweep = 8;  // channel tiles that share one sweep over a group's rows
+    static constexpr int kOut = 8;  // warps that turn sums into output
+    static constexpr int kThreads = 64 + 32 * kOut;
+    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kOut * kStoreBytes + 512;
 };
 
 template <bool I8, int BN>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
     product_pair_kernel(const Product p, const Layout lay, const __grid_constant__ CUtensorMap tm_a,
                         const __grid_constant__ CUtensorMap tm_b) {
     using Cfg = PairConfig<BN>;
@@ -676,7 +711,7 @@ __global__ void __launch_bounds__(192, 1)
     uint8_t *sA = smem;
     uint8_t *sB = sA + STAGES * kStageA;
     uint8_t *sStore = sB + STAGES * Cfg::kStageB;
-    uint64_t *full = reinterpret_cast<uint64_t *>(sStore + 4 * kStoreBytes);
+    uint64_t *full = reinterpret_cast<uint64_t *>(sStore + Cfg::kOut * kStoreBytes);
     uint64_t *empty = full + STAGES;
     uint64_t *tfull = empty + STAGES;
     uint64_t *tempty = tfull + 2;
@@ -698,7 +733,7 @@ __global__ void __launch_bounds__(192, 1)
         }
         for (int a = 0; a < 2; ++a) {
             emmy::mbar_init(&tfull[a], 1);
-            emmy::mbar_init(&tempty[a], 8);
+            emmy::mbar_init(&tempty[a], 2 * Cfg::kOut);
         }
         emmy::mbar_init(drain, 1);
         emmy::mbar_init(tail, 1);
@@ -714,33 +749,21 @@ __global__ void __launch_bounds__(192, 1)
             emmy::tma_prefetch(&tm_a);
             emmy::tma_prefetch(&tm_b);
         }
-        load_groups(g, p, BN);
     }
+    emmy::wait_for_prior_grid();
+    if (warp == 0) load_groups(g, p, BN);
     emmy::tc_fence_before();
     __syncthreads();
     emmy::cluster_sync();  // the peer signals the leader's barriers only after both are initialised
     emmy::tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
-    const int64_t mt = (p.m + 2 * kTileM - 1) / (2 * kTileM), total = mt * g.tiles[p.experts];
-    const int64_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    emmy::let_next_grid_start();
+    const int mt = static_cast<int>((p.m + 2 * kTileM - 1) / (2 * kTileM)), total = mt * g.tiles[p.experts];
+    const int pair = static_cast<int>(blockIdx.x >> 1), npairs = static_cast<int>(gridDim.x >> 1);
     int e = 0;
-
-    // Tile t: within an expert, kSweep channel tiles go over all of its rows together.
-    auto tile = [&](int64_t t) {
-        while (t >= mt * g.tiles[e + 1]) ++e;
-        const int begin = g.row[e], count = g.row[e + 1] - begin;
-        const int64_t ct = g.tiles[e + 1] - g.tiles[e], r = t - mt * g.tiles[e];
-        const int64_t sweep = r / (Cfg::kSweep * ct), in = r - sweep * Cfg::kSweep * ct;
-        const int64_t first = sweep * Cfg::kSweep, wide = min(static_cast<int64_t>(Cfg::kSweep), mt - first);
-        Tile o;
-        o.e = e;
-        o.begin = begin;
-        o.m0 = (first + in % wide) * 2 * kTileM + rank * kTileM;
-        o.c0 = in / wide * BN;
-        o.cols = static_cast<int>(min(static_cast<int64_t>(BN), (p.dw ? p.c : count) - o.c0));
-        o.kend = p.dw ? count : static_cast<int>(p.k);
-        o.kb0 = 0;
-        o.kb1 = o.kend / BK + (o.kend % BK != 0);
+    auto tile = [&](int t) {
+        Tile o = tile_at(p, g, t, mt, e, 2 * kTileM, BN, BK, 0, 1);
+        o.m0 += static_cast<int>(rank) * kTileM;  // this CTA's channels
         return o;
     };
 
@@ -750,9 +773,9 @@ __global__ void __launch_bounds__(192, 1)
         uint32_t peer_parity = 0u;  // of tail_peer, one bit for each stage
         uint32_t issued = 0u, parity_bits = 0u;
         bool ok = true;
-        for (int64_t t = pair; t < total && ok; t += npairs) {
+        for (int t = pair; t < total && ok; t += npairs) {
             const Tile w = tile(t);
-            const int m0 = static_cast<int>(w.m0), c0 = static_cast<int>(w.c0) + static_cast<int>(rank) * CN;
+            const int m0 = w.m0, c0 = w.c0 + static_cast<int>(rank) * CN;
             for (int kb = 0; kb < w.kb1; ++kb) {
                 if (!emmy::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
                     ok = false;
@@ -829,7 +852,7 @@ __global__ void __launch_bounds__(192, 1)
             const uint32_t peer_empty = emmy::mapa(&empty[0], 1);
             uint32_t stage = 0, phase = 0, it = 0;
             bool ok = true;
-            for (int64_t t = pair; t < total && ok; t += npairs, ++it) {
+            for (int t = pair; t < total && ok; t += npairs, ++it) {
                 const Tile w = tile(t);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
                 if (!emmy::mbar_wait_cluster(&tempty[acc], aphase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) break;
@@ -868,16 +891,17 @@ __global__ void __launch_bounds__(192, 1)
         __syncwarp();
     } else {
         // ---------------- output (both CTAs): own 128 channels of the tile
-        const int q = warp & 3;
+        const int q = warp & 3, part = (warp - 2) >> 2;
+        constexpr int SPAN = BN / (Cfg::kOut / 4);
         const uint32_t leader_tempty = emmy::mapa(&tempty[0], 0);
         uint32_t it = 0;
-        for (int64_t t = pair; t < total; t += npairs, ++it) {
+        for (int t = pair; t < total; t += npairs, ++it) {
             const Tile w = tile(t);
             const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
             if (!emmy::mbar_wait_cluster(&tfull[acc], aphase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)) break;
             emmy::tc_fence_after();
             store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
-                           sStore + q * kStoreBytes, lane);
+                           part * SPAN, (part + 1) * SPAN, sStore + (warp - 2) * kStoreBytes, lane);
             emmy::tc_fence_before();
             __syncwarp();
             if (lane == 0) emmy::mbar_arrive_cluster(leader_tempty + acc * 8u);
