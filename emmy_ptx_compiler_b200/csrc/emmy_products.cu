@@ -304,43 +304,63 @@ cudaLaunchAttribute early_start() {
     return attr;
 }
 
-using TcKernel = void (*)(Product, Layout, CUtensorMap, CUtensorMap);
+using TcKernel = void (*)(Product, bool, CUtensorMap, CUtensorMap);
 
-// A launch of clusters of `cluster` CTAs.  `ready` marks the devices on which the kernel's
-// shared-memory limit has been raised.
-int launch_clusters(const Call &call, TcKernel kernel, std::atomic<uint64_t> &ready, const Product &p, const Layout &lay,
-                    const CUtensorMap &ta, const CUtensorMap &tb, int64_t clusters, int cluster, int threads,
-                    uint32_t smem) {
-    if (!(ready.load(std::memory_order_acquire) >> call.dev & 1)) {
+// What every variant's launch takes.
+struct Launch {
+    const Call &call;
+    const Product &p;
+    bool bf16;
+    const CUtensorMap &ta, &tb;
+    int64_t clusters;
+    int cluster;
+};
+
+// `ready` marks the devices on which the kernel's shared-memory limit has been raised.
+int launch_clusters(const Launch &l, TcKernel kernel, std::atomic<uint64_t> &ready, int threads, uint32_t smem) {
+    if (!(ready.load(std::memory_order_acquire) >> l.call.dev & 1)) {
         const cudaError_t err =
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (err != cudaSuccess) return launched(call, err);
-        ready.fetch_or(1ull << call.dev, std::memory_order_release);
+        if (err != cudaSuccess) return launched(l.call, err);
+        ready.fetch_or(1ull << l.call.dev, std::memory_order_release);
     }
-    cudaLaunchConfig_t cfg = config(call, clusters * cluster, threads, smem);
+    cudaLaunchConfig_t cfg = config(l.call, l.clusters * l.cluster, threads, smem);
     cudaLaunchAttribute attrs[2] = {early_start(), {}};
     attrs[1].id = cudaLaunchAttributeClusterDimension;
-    attrs[1].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    attrs[1].val.clusterDim = {static_cast<unsigned>(l.cluster), 1, 1};
     cfg.attrs = attrs;
     cfg.numAttrs = 2;
-    return launched(call, cudaLaunchKernelEx(&cfg, kernel, p, lay, ta, tb));
+    return launched(l.call, cudaLaunchKernelEx(&cfg, kernel, l.p, l.bf16, l.ta, l.tb));
 }
 
-template <bool I8, int BN, bool TMA>
-int launch_single(const Call &call, const Product &p, const Layout &lay, const CUtensorMap &ta, const CUtensorMap &tb,
-                  int64_t clusters, int split) {
+template <bool I8, int LAYOUT, int BN, bool TMA>
+int launch_single(const Launch &l) {
     using Cfg = TcConfig<I8, BN, TMA>;
     static std::atomic<uint64_t> ready{0};
-    return launch_clusters(call, product_tc_kernel<I8, BN, TMA>, ready, p, lay, ta, tb, clusters, split, Cfg::kThreads,
-                           Cfg::kSmem);
+    return launch_clusters(l, product_tc_kernel<I8, LAYOUT, BN, TMA>, ready, Cfg::kThreads, Cfg::kSmem);
 }
 
-template <bool I8, int BN>
-int launch_pair(const Call &call, const Product &p, const Layout &lay, const CUtensorMap &ta, const CUtensorMap &tb,
-                int64_t pairs) {
+template <bool I8, int LAYOUT, int BN>
+int launch_pair(const Launch &l) {
+    using Cfg = PairConfig<BN>;
     static std::atomic<uint64_t> ready{0};
-    return launch_clusters(call, product_pair_kernel<I8, BN>, ready, p, lay, ta, tb, pairs, 2,
-                           PairConfig<BN>::kThreads, PairConfig<BN>::kSmem);
+    return launch_clusters(l, product_pair_kernel<I8, LAYOUT, BN>, ready, Cfg::kThreads, Cfg::kSmem);
+}
+
+template <bool I8, int LAYOUT>
+int launch_variant(const Launch &l, bool tma, int pair, int bn) {
+    if (pair) return pair == 256 ? launch_pair<I8, LAYOUT, 256>(l) : launch_pair<I8, LAYOUT, 128>(l);
+    if constexpr (LAYOUT == kMM) {
+        return tma ? launch_single<I8, LAYOUT, 128, true>(l) : launch_single<I8, LAYOUT, 128, false>(l);
+    } else {
+        if (!tma) return bn <= 32 ? launch_single<I8, LAYOUT, 32, false>(l) : launch_single<I8, LAYOUT, 128, false>(l);
+        switch (bn) {
+            case 16: return launch_single<I8, LAYOUT, 16, true>(l);
+            case 32: return launch_single<I8, LAYOUT, 32, true>(l);
+            case 64: return launch_single<I8, LAYOUT, 64, true>(l);
+            default: return launch_single<I8, LAYOUT, 128, true>(l);
+        }
+    }
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -355,16 +375,13 @@ const void *end_of(const Operand &o, int esize) {
 template <bool I8>
 int launch_product(const Call &call, Product p, bool bf16) {
     constexpr int esize = I8 ? 1 : 2, bk = 128 / esize;
-    Layout lay{};
-    lay.a_mn = p.dw || p.a_k != 1;
-    lay.b_mn = p.dw;
-    lay.bf16 = bf16;
+    const bool a_mn = p.dw || p.a_k != 1;
     Operand a{p.a, 0, 0, 0, 1, 0}, b{p.b, 0, 0, 0, 1, 0};
     if (p.dw) {
         a.inner = p.m, a.rows = p.rows, a.row_stride = p.a_k;
         b.inner = p.c, b.rows = p.rows, b.row_stride = p.b_k;
     } else {
-        a.inner = lay.a_mn ? p.m : p.k, a.rows = lay.a_mn ? p.k : p.m, a.row_stride = lay.a_mn ? p.a_k : p.a_m;
+        a.inner = a_mn ? p.m : p.k, a.rows = a_mn ? p.k : p.m, a.row_stride = a_mn ? p.a_k : p.a_m;
         a.mats = p.experts, a.mat_stride = p.a_e;
         b.inner = p.k, b.rows = p.rows, b.row_stride = p.b_c;
     }
@@ -397,29 +414,24 @@ int launch_product(const Call &call, Product p, bool bf16) {
         const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                          : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-        if (!encode(&ta, a, type, esize, 3, bk, lay.a_mn ? 64 : kTileM) ||
-            !encode(&tb, b, type, esize, 2, bk, lay.b_mn ? 64 : pair ? pair / 2 : bn))
+        if (!encode(&ta, a, type, esize, 3, bk, a_mn ? 64 : kTileM) ||
+            !encode(&tb, b, type, esize, 2, bk, p.dw ? 64 : pair ? pair / 2 : bn))
             return report(EMMY_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", call.name);
     }
-    if (pair) {
-        int64_t pairs = most(256, pair);
-        if (pairs > kSms / 2) pairs = kSms / 2;
-        return pair == 256 ? launch_pair<I8, 256>(call, p, lay, ta, tb, pairs)
-                           : launch_pair<I8, 128>(call, p, lay, ta, tb, pairs);
-    }
-    const int resident = kSms * (tma && bn <= 32 ? 2 : 1);
+    const int resident = pair ? kSms : kSms * (tma && bn <= 32 ? 2 : 1);
     int split = 1;
-    while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident && kblocks >= split * 2 * 4) split *= 2;
-    int64_t clusters = most(kTileM, bn);
-    if (clusters > resident / split) clusters = resident / split;
-    if (!tma)
-        return bn <= 32 ? launch_single<I8, 32, false>(call, p, lay, ta, tb, clusters, split)
-                        : launch_single<I8, 128, false>(call, p, lay, ta, tb, clusters, split);
-    switch (bn) {
-        case 16: return launch_single<I8, 16, true>(call, p, lay, ta, tb, clusters, split);
-        case 32: return launch_single<I8, 32, true>(call, p, lay, ta, tb, clusters, split);
-        case 64: return launch_single<I8, 64, true>(call, p, lay, ta, tb, clusters, split);
-        default: return launch_single<I8, 128, true>(call, p, lay, ta, tb, clusters, split);
+    if (!pair)
+        while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident && kblocks >= split * 2 * 4) split *= 2;
+    const int cluster = pair ? 2 : split;
+    int64_t clusters = pair ? most(2 * kTileM, pair) : most(kTileM, bn);
+    if (clusters > resident / cluster) clusters = resident / cluster;
+    const Launch l{call, p, bf16, ta, tb, clusters, cluster};
+    if constexpr (I8) {
+        return launch_variant<true, kKK>(l, tma, pair, bn);
+    } else {
+        return p.dw ? launch_variant<false, kMM>(l, tma, pair, bn)
+               : a_mn ? launch_variant<false, kMK>(l, tma, pair, bn)
+                      : launch_variant<false, kKK>(l, tma, pair, bn);
     }
 }
 

@@ -116,10 +116,45 @@ constexpr uint32_t kBlockBytes = 128;                  // one 128-byte swizzle r
 constexpr uint32_t kPanel = 64 * kBlockBytes;          // 64 k x 64 m (or c) of an MN-major 16-bit operand
 constexpr uint32_t kStageA = kTileM * kBlockBytes;
 
-// What a launch passes beside the product: the operands' layouts.
-struct Layout {
-    bool a_mn, b_mn;  // contiguous along m (c) instead of k
-    bool bf16;
+// The operands' layouts: which of them are contiguous along m (c) instead of along k.
+enum : int { kKK = 0, kMK = 1, kMM = 2 };  // kMM: dw
+
+// One block's MMAs (128 bytes of k, or the first `steps` quarters of it) over the operands whose
+// descriptors for stage 0 are `a`, `b`.  The stage and the quarter only add to the descriptors' low
+// words, and everything else is known at compile time: a single thread issues all of this, and a
+// block of 256 x 256 leaves it 512 clocks.
+template <bool I8, int LAYOUT, bool PAIR>
+struct Issue {
+    static constexpr bool kAmn = LAYOUT != kKK, kBmn = LAYOUT == kMM;
+    static constexpr uint32_t kStepA = (kAmn ? 16 * kBlockBytes : 32) >> 4, kStepB = (kBmn ? 16 * kBlockBytes : 32) >> 4;
+
+    uint32_t a_lo, b_lo, a_hi, b_hi, idesc;
+
+    __device__ __forceinline__ Issue(const uint8_t *a, const uint8_t *b, bool bf16, int n) {
+        const uint64_t da = emmy::smem_desc_sw128(emmy::smem_u32(a), kAmn ? kPanel : 16, 1024);
+        const uint64_t db = emmy::smem_desc_sw128(emmy::smem_u32(b), kBmn ? kPanel : 16, 1024);
+        a_lo = static_cast<uint32_t>(da), a_hi = static_cast<uint32_t>(da >> 32);
+        b_lo = static_cast<uint32_t>(db), b_hi = static_cast<uint32_t>(db >> 32);
+        const uint32_t m = PAIR ? 2 * kTileM : kTileM;
+        idesc = I8 ? emmy::idesc_s8(m, n) : emmy::idesc_f16_major(bf16 ? 1u : 0u, kAmn, kBmn, m, n);
+    }
+    __device__ __forceinline__ void mma(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t more) const {
+        const uint64_t ad = static_cast<uint64_t>(a_hi) << 32 | a, bd = static_cast<uint64_t>(b_hi) << 32 | b;
+        if constexpr (I8 && PAIR) emmy::umma_i8_pair(d_tmem, ad, bd, idesc, more);
+        else if constexpr (I8) emmy::umma_i8(d_tmem, ad, bd, idesc, more);
+        else if constexpr (PAIR) emmy::umma_f16_pair(d_tmem, ad, bd, idesc, more);
+        else emmy::umma_f16(d_tmem, ad, bd, idesc, more);
+    }
+    __device__ __forceinline__ void block(uint32_t d_tmem, uint32_t a_off, uint32_t b_off, uint32_t more, int steps) const {
+        const uint32_t a = a_lo + (a_off >> 4), b = b_lo + (b_off >> 4);
+        if (LAYOUT != kMM || steps == 4) {
+            mma(d_tmem, a, b, more);
+            #pragma unroll
+            for (int kk = 1; kk < 4; ++kk) mma(d_tmem, a + kk * kStepA, b + kk * kStepB, 1u);
+        } else {
+            for (int kk = 0; kk < steps; ++kk) mma(d_tmem, a + kk * kStepA, b + kk * kStepB, more | (kk > 0));
+        }
+    }
 };
 
 struct Tile {
@@ -374,12 +409,13 @@ struct TcConfig {
 // turn the other into output, 4 or 8 of them: a warp reaches 32 of the 128 lanes.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
 // added in rank order through distributed shared memory, each CTA finishing its share of columns:
 // the result depends on neither timing nor the number of SMs.
-template <bool I8, int BN, bool TMA>
+template <bool I8, int LAYOUT, int BN, bool TMA>
 __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
-    product_tc_kernel(const Product p, const Layout lay, const __grid_constant__ CUtensorMap tm_a,
+    product_tc_kernel(const Product p, const bool bf16, const __grid_constant__ CUtensorMap tm_a,
                       const __grid_constant__ CUtensorMap tm_b) {
     using Cfg = TcConfig<I8, BN, TMA>;
     using T = std::conditional_t<I8, int8_t, uint16_t>;
+    static_assert(LAYOUT != kMM || BN % 64 == 0, "dw's B comes in panels of 64");
     constexpr int STAGES = Cfg::kStages;
     constexpr int BK = I8 ? 128 : 64;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -443,7 +479,6 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
             if (lane == 0) {
                 for (int t = first; t < last && ok; t += step) {
                     const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
-                    const int m0 = w.m0, c0 = w.c0;
                     for (int kb = w.kb0; kb < w.kb1; ++kb) {
                         if (!emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
                             ok = false;
@@ -452,18 +487,19 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                         emmy::mbar_arrive_expect_tx(&full[stage], Cfg::kStage);
                         uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
                         const int k0 = kb * BK;
-                        if (lay.a_mn) {
-                            const int ka = p.dw ? w.begin + k0 : k0, ez = p.dw ? 0 : w.e;
-                            emmy::tma_load_3d(a, &tm_a, &full[stage], m0, ka, ez);
-                            emmy::tma_load_3d(a + kPanel, &tm_a, &full[stage], m0 + 64, ka, ez);
+                        if constexpr (LAYOUT == kKK) {
+                            emmy::tma_load_3d(a, &tm_a, &full[stage], k0, w.m0, w.e);
                         } else {
-                            emmy::tma_load_3d(a, &tm_a, &full[stage], k0, m0, w.e);
+                            const int ka = LAYOUT == kMM ? w.begin + k0 : k0, ez = LAYOUT == kMM ? 0 : w.e;
+                            emmy::tma_load_3d(a, &tm_a, &full[stage], w.m0, ka, ez);
+                            emmy::tma_load_3d(a + kPanel, &tm_a, &full[stage], w.m0 + 64, ka, ez);
                         }
-                        if (lay.b_mn) {
+                        if constexpr (LAYOUT == kMM) {
+                            #pragma unroll
                             for (int j = 0; j < BN / 64; ++j)
-                                emmy::tma_load_2d(b + j * kPanel, &tm_b, &full[stage], c0 + 64 * j, w.begin + k0);
+                                emmy::tma_load_2d(b + j * kPanel, &tm_b, &full[stage], w.c0 + 64 * j, w.begin + k0);
                         } else {
-                            emmy::tma_load_2d(b, &tm_b, &full[stage], k0, w.begin + c0);
+                            emmy::tma_load_2d(b, &tm_b, &full[stage], k0, w.begin + w.c0);
                         }
                         issued |= 1u << stage;
                         parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
@@ -493,7 +529,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                 auto load = [&](int kb) {
                     const int64_t k0 = static_cast<int64_t>(kb) * BK, kleft = w.kend - k0;
                     const int64_t row = th >> 1, krow = row & 63, panel = row >> 6;
-                    if (lay.a_mn) {
+                    if constexpr (LAYOUT != kKK) {
                         const int64_t m = w.m0 + 64 * panel;
                         pa = reinterpret_cast<const uint8_t *>(ae + (k0 + krow) * p.a_k + m);
                         na = krow < kleft ? (p.m - m) * static_cast<int64_t>(sizeof(T)) : 0;
@@ -505,7 +541,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                     na -= 64 * half;
                     load_unit(ua, pa, na, a_lo, a_hi);
                     if (!has_b) return;
-                    if (lay.b_mn) {
+                    if constexpr (LAYOUT == kMM) {
                         pb = reinterpret_cast<const uint8_t *>(be + (k0 + krow) * p.b_k + w.c0 + 64 * panel);
                         nb = krow < kleft ? (w.cols - 64 * panel) * static_cast<int64_t>(sizeof(T)) : 0;
                     } else {
@@ -536,11 +572,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                 }
             }
         } else if (warp == 1) {
-            const uint32_t idesc = I8 ? emmy::idesc_s8(kTileM, BN)
-                                      : emmy::idesc_f16_major(lay.bf16 ? 1u : 0u, lay.a_mn, lay.b_mn, kTileM, BN);
-            // one MMA takes 32 bytes of k: along a swizzled row when k is contiguous, else 16 rows further
-            const uint32_t a_step = lay.a_mn ? 16 * kBlockBytes : 32, a_lbo = lay.a_mn ? kPanel : 16;
-            const uint32_t b_step = lay.b_mn ? 16 * kBlockBytes : 32, b_lbo = lay.b_mn ? kPanel : 16;
+            const Issue<I8, LAYOUT, false> issue(sA, sB, bf16, BN);
             for (int t = first; t < last && ok; t += step, ++it) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
@@ -555,14 +587,14 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                         ok = false;
                         break;
                     }
-                    uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
                     int steps = 4;
-                    if (p.dw && w.kend - kb * BK < BK) {
+                    if (LAYOUT == kMM && w.kend - kb * BK < BK) {
                         // the block ends inside: later rows belong to the next group (or hold
                         // anything), so what the last MMA takes of them becomes zero in both operands
                         const int have = w.kend - kb * BK;
                         steps = (have + 15) / 16;
                         if (TMA) {
+                            uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
                             for (int j = 0; j < 2; ++j) zero_panel_rows(a + j * kPanel, have, steps * 16, lane);
                             for (int j = 0; j < BN / 64; ++j) zero_panel_rows(b + j * kPanel, have, steps * 16, lane);
                             emmy::fence_proxy_async();
@@ -571,14 +603,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                     }
                     emmy::tc_fence_after();
                     if (lane == 0) {
-                        const uint32_t a_base = emmy::smem_u32(a), b_base = emmy::smem_u32(b);
-                        for (int kk = 0; kk < steps; ++kk) {
-                            const uint64_t ad = emmy::smem_desc_sw128(a_base + kk * a_step, a_lbo, 1024);
-                            const uint64_t bd = emmy::smem_desc_sw128(b_base + kk * b_step, b_lbo, 1024);
-                            const uint32_t more = (kb > w.kb0 || kk > 0) ? 1u : 0u;
-                            if constexpr (I8) emmy::umma_i8(d_tmem, ad, bd, idesc, more);
-                            else emmy::umma_f16(d_tmem, ad, bd, idesc, more);
-                        }
+                        issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, kb > w.kb0, steps);
                         emmy::umma_commit(&empty[stage]);
                     }
                     __syncwarp();
@@ -699,9 +724,9 @@ struct PairConfig {
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kOut * kStoreBytes + 512;
 };
 
-template <bool I8, int BN>
+template <bool I8, int LAYOUT, int BN>
 __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
-    product_pair_kernel(const Product p, const Layout lay, const __grid_constant__ CUtensorMap tm_a,
+    product_pair_kernel(const Product p, const bool bf16, const __grid_constant__ CUtensorMap tm_a,
                         const __grid_constant__ CUtensorMap tm_b) {
     using Cfg = PairConfig<BN>;
     constexpr int STAGES = Cfg::kStages, BK = I8 ? 128 : 64, CN = BN / 2;
@@ -773,66 +798,88 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
         uint32_t peer_parity = 0u;  // of tail_peer, one bit for each stage
         uint32_t issued = 0u, parity_bits = 0u;
         bool ok = true;
+        const uint32_t leader_full = emmy::mapa(&full[0], 0), own_tail = emmy::mapa(tail, rank);
+        // One block's loads, completing on the barrier at cluster address `bar`; one thread.
+        auto load = [&](const Tile &w, int kb, uint32_t bar) {
+            uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
+            const int k0 = kb * BK, c0 = w.c0 + static_cast<int>(rank) * CN;
+            if constexpr (LAYOUT == kKK) {
+                emmy::tma_load_3d_pair(a, &tm_a, bar, k0, w.m0, w.e);
+            } else {
+                const int ka = LAYOUT == kMM ? w.begin + k0 : k0, ez = LAYOUT == kMM ? 0 : w.e;
+                emmy::tma_load_3d_pair(a, &tm_a, bar, w.m0, ka, ez);
+                emmy::tma_load_3d_pair(a + kPanel, &tm_a, bar, w.m0 + 64, ka, ez);
+            }
+            if constexpr (LAYOUT == kMM) {
+                #pragma unroll
+                for (int j = 0; j < CN / 64; ++j)
+                    emmy::tma_load_2d_pair(b + j * kPanel, &tm_b, bar, c0 + 64 * j, w.begin + k0);
+            } else {
+                emmy::tma_load_2d_pair(b, &tm_b, bar, k0, w.begin + c0);
+            }
+        };
+        auto next = [&]() {
+            if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        };
         for (int t = pair; t < total && ok; t += npairs) {
             const Tile w = tile(t);
-            const int m0 = w.m0, c0 = w.c0 + static_cast<int>(rank) * CN;
-            for (int kb = 0; kb < w.kb1; ++kb) {
-                if (!emmy::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
-                    ok = false;
-                    break;
+            const int whole = LAYOUT == kMM ? w.kend / BK : w.kb1;
+            if (lane == 0) {
+                for (int kb = 0; kb < whole; ++kb) {
+                    if (!emmy::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) {
+                        emmy::mbar_arrive_expect_tx(&full[stage], 2u * Cfg::kStage);
+                        issued |= 1u << stage;
+                        parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
+                    }
+                    load(w, kb, leader_full + stage * 8u);
+                    next();
                 }
-                uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
-                const int k0 = kb * BK, have = w.kend - k0;
-                const bool ends_inside = p.dw && have < BK;
+            }
+            if constexpr (LAYOUT == kMM) {
+                // A last block that ends inside: later rows belong to the next group (or hold
+                // anything), and what the last MMA takes of them becomes zero in both operands
+                // before the leader's barrier completes.  The whole warp does that.
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                stage = __shfl_sync(0xffffffffu, stage, 0);
+                phase = __shfl_sync(0xffffffffu, phase, 0);
+                if (whole == w.kb1) continue;
+                ok = emmy::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
                 if (lane == 0) {
-                    if (ends_inside) emmy::mbar_arrive_expect_tx(tail, Cfg::kStage);
-                    else if (rank == 0) emmy::mbar_arrive_expect_tx(&full[stage], 2u * Cfg::kStage);
-                    const uint32_t bar = ends_inside ? emmy::mapa(tail, rank) : emmy::mapa(&full[stage], 0);
-                    if (lay.a_mn) {
-                        const int ka = p.dw ? w.begin + k0 : k0, ez = p.dw ? 0 : w.e;
-                        emmy::tma_load_3d_pair(a, &tm_a, bar, m0, ka, ez);
-                        emmy::tma_load_3d_pair(a + kPanel, &tm_a, bar, m0 + 64, ka, ez);
-                    } else {
-                        emmy::tma_load_3d_pair(a, &tm_a, bar, k0, m0, w.e);
-                    }
-                    if (lay.b_mn) {
-                        for (int j = 0; j < CN / 64; ++j)
-                            emmy::tma_load_2d_pair(b + j * kPanel, &tm_b, bar, c0 + 64 * j, w.begin + k0);
-                    } else {
-                        emmy::tma_load_2d_pair(b, &tm_b, bar, k0, w.begin + c0);
-                    }
+                    emmy::mbar_arrive_expect_tx(tail, Cfg::kStage);
+                    load(w, whole, own_tail);
                 }
                 __syncwarp();
-                if (ends_inside) {
-                    // later rows belong to the next group (or hold anything): what the last MMA takes
-                    // of them becomes zero in both operands before the leader's barrier completes
-                    ok = emmy::mbar_wait_cluster(tail, tails & 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
+                ok = emmy::mbar_wait_cluster(tail, tails & 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ++tails;
+                const int have = w.kend - whole * BK, upto = (have + 15) / 16 * 16;
+                for (int j = 0; j < 2; ++j) zero_panel_rows(sA + stage * kStageA + j * kPanel, have, upto, lane);
+                for (int j = 0; j < CN / 64; ++j)
+                    zero_panel_rows(sB + stage * Cfg::kStageB + j * kPanel, have, upto, lane);
+                emmy::fence_proxy_async();
+                __syncwarp();
+                if (rank == 1) {
+                    if (lane == 0) emmy::mbar_arrive_cluster(emmy::mapa(&tail_peer[stage], 0));
+                } else {
+                    ok = emmy::mbar_wait_cluster(&tail_peer[stage], peer_parity >> stage & 1u, abort_flag,
+                                                 EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    const int upto = (have + 15) / 16 * 16;
-                    for (int j = 0; j < 2; ++j) zero_panel_rows(a + j * kPanel, have, upto, lane);
-                    for (int j = 0; j < CN / 64; ++j) zero_panel_rows(b + j * kPanel, have, upto, lane);
-                    emmy::fence_proxy_async();
-                    __syncwarp();
-                    if (rank == 1) {
-                        if (lane == 0) emmy::mbar_arrive_cluster(emmy::mapa(&tail_peer[stage], 0));
-                    } else {
-                        ok = emmy::mbar_wait_cluster(&tail_peer[stage], peer_parity >> stage & 1u, abort_flag,
-                                                     EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
-                        peer_parity ^= 1u << stage;
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        if (lane == 0) emmy::mbar_arrive(&full[stage]);
-                    }
-                    ++tails;
-                } else if (rank == 0) {
-                    issued |= 1u << stage;
-                    parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
+                    peer_parity ^= 1u << stage;
+                    if (lane == 0) emmy::mbar_arrive(&full[stage]);
                 }
-                if (++stage == STAGES) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
+                next();
             }
         }
         if (!ok && rank == 0 && lane == 0) {
@@ -845,11 +892,8 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
     } else if (warp == 1) {
         if (rank == 0 && lane == 0) {
             // ---------------- MMA issuer (leader only)
-            const uint32_t idesc = I8 ? emmy::idesc_s8(2 * kTileM, BN)
-                                      : emmy::idesc_f16_major(lay.bf16 ? 1u : 0u, lay.a_mn, lay.b_mn, 2 * kTileM, BN);
-            const uint32_t a_step = lay.a_mn ? 16 * kBlockBytes : 32, a_lbo = lay.a_mn ? kPanel : 16;
-            const uint32_t b_step = lay.b_mn ? 16 * kBlockBytes : 32, b_lbo = lay.b_mn ? kPanel : 16;
-            const uint32_t peer_empty = emmy::mapa(&empty[0], 1);
+            const Issue<I8, LAYOUT, true> issue(sA, sB, bf16, BN);
+            const uint32_t peer_empty = emmy::mapa(&empty[0], 1), peer_tfull = emmy::mapa(&tfull[0], 1);
             uint32_t stage = 0, phase = 0, it = 0;
             bool ok = true;
             for (int t = pair; t < total && ok; t += npairs, ++it) {
@@ -864,15 +908,8 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
                         break;
                     }
                     emmy::tc_fence_after();
-                    const uint32_t a_base = emmy::smem_u32(sA + stage * kStageA);
-                    const uint32_t b_base = emmy::smem_u32(sB + stage * Cfg::kStageB);
-                    const int have = w.kend - kb * BK, steps = p.dw && have < BK ? (have + 15) / 16 : 4;
-                    for (int kk = 0; kk < steps; ++kk) {
-                        const uint64_t ad = emmy::smem_desc_sw128(a_base + kk * a_step, a_lbo, 1024);
-                        const uint64_t bd = emmy::smem_desc_sw128(b_base + kk * b_step, b_lbo, 1024);
-                        if constexpr (I8) emmy::umma_i8_pair(d_tmem, ad, bd, idesc, (kb | kk) != 0 ? 1u : 0u);
-                        else emmy::umma_f16_pair(d_tmem, ad, bd, idesc, (kb | kk) != 0 ? 1u : 0u);
-                    }
+                    const int have = w.kend - kb * BK;
+                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, kb > 0, have < BK ? (have + 15) / 16 : 4);
                     emmy::umma_commit_pair(emmy::smem_u32(&empty[stage]));
                     emmy::umma_commit_pair(peer_empty + stage * 8u);
                     if (++stage == STAGES) {
@@ -882,7 +919,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
                 }
                 if (!ok) break;
                 emmy::umma_commit_pair(emmy::smem_u32(&tfull[acc]));
-                emmy::umma_commit_pair(emmy::mapa(&tfull[acc], 1));
+                emmy::umma_commit_pair(peer_tfull + acc * 8u);
             }
             // arrives on both CTAs once every pair MMA has finished
             emmy::umma_commit_pair(emmy::smem_u32(drain));
