@@ -13,14 +13,43 @@
 
 namespace emmy {
 
-// D[tmem] (+)= A[smem] x B[smem], kind::i8, one CTA.
-__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                        uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+// tcgen05.mma and tcgen05.commit predicated on `elected`, for a warp that runs its loop together and
+// issues from one lane.  The operands have to be in uniform registers: they stay there while the
+// control flow is the whole warp's, and have to be moved there for each instruction inside a
+// branch that one lane takes.
+template <bool I8, bool PAIR>
+__device__ __forceinline__ void umma_if(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+#define EMMY_UMMA_IF(GROUP, KIND)                                                              \
+    asm volatile(                                                                              \
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"               \
+        " @q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n}\n" ::"r"( \
+            d_tmem),                                                                           \
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)                    \
+        : "memory")
+    if constexpr (I8 && PAIR) EMMY_UMMA_IF("2", "i8");
+    else if constexpr (I8) EMMY_UMMA_IF("1", "i8");
+    else if constexpr (PAIR) EMMY_UMMA_IF("2", "f16");
+    else EMMY_UMMA_IF("1", "f16");
+#undef EMMY_UMMA_IF
+}
+
+// Arrive on this CTA's `bar` (PAIR: on the barrier at that place of both CTAs) once every MMA issued
+// before has completed.
+template <bool PAIR>
+__device__ __forceinline__ void umma_commit_if(uint32_t elected, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+            " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n}\n"
+            ::"r"(bar), "r"(elected), "h"(static_cast<uint16_t>(3))
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+            " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+            "r"(elected)
+            : "memory");
 }
 
 // 32 lanes x 16 consecutive 32-bit columns.
@@ -50,16 +79,6 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t smem_addr, uint32_t a
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_addr), "r"(a),
                  "r"(b), "r"(c), "r"(d)
                  : "memory");
-}
-
-// D[tmem of both CTAs] (+)= A x B over both CTAs' shared memory, kind::i8; issued by the leader.
-__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                             uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
 }
 
 // 3-D tiled load into this CTA's shared memory, completion counted on the mbarrier at
@@ -128,23 +147,22 @@ struct Issue {
     static constexpr bool kAmn = LAYOUT != kKK, kBmn = LAYOUT == kMM;
     static constexpr uint32_t kStepA = (kAmn ? 16 * kBlockBytes : 32) >> 4, kStepB = (kBmn ? 16 * kBlockBytes : 32) >> 4;
 
-    uint32_t a_lo, b_lo, a_hi, b_hi, idesc;
+    uint32_t a_lo, b_lo, a_hi, b_hi, idesc, elected;
 
     __device__ __forceinline__ Issue(const uint8_t *a, const uint8_t *b, bool bf16, int n) {
         const uint64_t da = emmy::smem_desc_sw128(emmy::smem_u32(a), kAmn ? kPanel : 16, 1024);
         const uint64_t db = emmy::smem_desc_sw128(emmy::smem_u32(b), kBmn ? kPanel : 16, 1024);
         a_lo = static_cast<uint32_t>(da), a_hi = static_cast<uint32_t>(da >> 32);
         b_lo = static_cast<uint32_t>(db), b_hi = static_cast<uint32_t>(db >> 32);
+        elected = emmy::elect_one();
         const uint32_t m = PAIR ? 2 * kTileM : kTileM;
         idesc = I8 ? emmy::idesc_s8(m, n) : emmy::idesc_f16_major(bf16 ? 1u : 0u, kAmn, kBmn, m, n);
     }
     __device__ __forceinline__ void mma(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t more) const {
-        const uint64_t ad = static_cast<uint64_t>(a_hi) << 32 | a, bd = static_cast<uint64_t>(b_hi) << 32 | b;
-        if constexpr (I8 && PAIR) emmy::umma_i8_pair(d_tmem, ad, bd, idesc, more);
-        else if constexpr (I8) emmy::umma_i8(d_tmem, ad, bd, idesc, more);
-        else if constexpr (PAIR) emmy::umma_f16_pair(d_tmem, ad, bd, idesc, more);
-        else emmy::umma_f16(d_tmem, ad, bd, idesc, more);
+        emmy::umma_if<I8, PAIR>(elected, d_tmem, static_cast<uint64_t>(a_hi) << 32 | a,
+                                static_cast<uint64_t>(b_hi) << 32 | b, idesc, more);
     }
+    // the whole warp calls these
     __device__ __forceinline__ void block(uint32_t d_tmem, uint32_t a_off, uint32_t b_off, uint32_t more, int steps) const {
         const uint32_t a = a_lo + (a_off >> 4), b = b_lo + (b_off >> 4);
         if (LAYOUT != kMM || steps == 4) {
@@ -155,7 +173,13 @@ struct Issue {
             for (int kk = 0; kk < steps; ++kk) mma(d_tmem, a + kk * kStepA, b + kk * kStepB, more | (kk > 0));
         }
     }
+    __device__ __forceinline__ void commit(uint64_t *bar) const {
+        emmy::umma_commit_if<PAIR>(elected, emmy::smem_u32(bar));
+    }
 };
+
+// A value that is the same on every lane, in a form the compiler knows to be.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 struct Tile {
     int e, begin;   // expert and its first row
@@ -164,6 +188,12 @@ struct Tile {
     int kend;       // extent of the sum
     int kb0, kb1;   // blocks of it that this CTA sums
 };
+
+// MMAs (of 16 k) in the block before kb1: 4, or those up to the end of the sum.
+__device__ __forceinline__ int last_block_steps(const Tile &w, int kb1, int bk) {
+    const int have = w.kend - (kb1 - 1) * bk;
+    return have < bk ? (have + 15) / 16 : 4;
+}
 
 // Channel tiles that go over all rows of their expert together: what they read of the rows stays
 // in L2 from one to the next.
@@ -576,46 +606,41 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
             for (int t = first; t < last && ok; t += step, ++it) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
-                if (!emmy::mbar_wait(&tempty[acc], aphase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) {
-                    ok = false;
-                    break;
-                }
+                ok = __all_sync(0xffffffffu, emmy::mbar_wait(&tempty[acc], aphase ^ 1u, abort_flag,
+                                                             EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
+                if (!ok) break;
                 emmy::tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * BN;
-                for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    if (!emmy::mbar_wait(&full[stage], phase, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) {
-                        ok = false;
-                        break;
-                    }
-                    int steps = 4;
-                    if (LAYOUT == kMM && w.kend - kb * BK < BK) {
-                        // the block ends inside: later rows belong to the next group (or hold
+                const int blocks = uniform(w.kb1 - w.kb0), last_steps = uniform(last_block_steps(w, w.kb1, BK));
+                for (int i = 0; i < blocks; ++i) {
+                    ok = __all_sync(0xffffffffu, emmy::mbar_wait(&full[stage], phase, abort_flag,
+                                                                 EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
+                    if (!ok) break;
+                    const int steps = LAYOUT == kMM && i == blocks - 1 ? last_steps : 4;
+                    if (LAYOUT == kMM && TMA && i == blocks - 1) {
+                        // a block that ends inside: later rows belong to the next group (or hold
                         // anything), so what the last MMA takes of them becomes zero in both operands
-                        const int have = w.kend - kb * BK;
-                        steps = (have + 15) / 16;
-                        if (TMA) {
+                        const int have = min(BK, w.kend - (w.kb1 - 1) * BK);
+                        if (have < steps * 16) {
                             uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
                             for (int j = 0; j < 2; ++j) zero_panel_rows(a + j * kPanel, have, steps * 16, lane);
                             for (int j = 0; j < BN / 64; ++j) zero_panel_rows(b + j * kPanel, have, steps * 16, lane);
                             emmy::fence_proxy_async();
-                            __syncwarp();
                         }
+                        __syncwarp();
                     }
                     emmy::tc_fence_after();
-                    if (lane == 0) {
-                        issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, kb > w.kb0, steps);
-                        emmy::umma_commit(&empty[stage]);
-                    }
-                    __syncwarp();
+                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, i > 0, steps);
+                    issue.commit(&empty[stage]);
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                if (lane == 0) emmy::umma_commit(&tfull[acc]);
-                __syncwarp();
+                issue.commit(&tfull[acc]);
             }
+            __syncwarp();
         } else if (warp >= 2 && warp < 2 + Cfg::kOut) {
             const int q = warp & 3, part = (warp - 2) >> 2;
             constexpr int PARTS = Cfg::kOut / 4, SPAN = BN / PARTS;
@@ -692,11 +717,13 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
         for (int s = 0; s < STAGES; ++s)
             if (issued & (1u << s)) emmy::mbar_wait(&full[s], (parity_bits >> s) & 1u, &never, 0u, 20000000ull);
     }
-    if (warp == 1 && lane == 0) {
-        // every MMA has finished before tensor memory is released (bounded)
-        emmy::umma_commit(drain);
+    if (warp == 1) {
+        // every MMA has finished before tensor memory is released (bounded); committed by the lane
+        // that issued them
+        emmy::umma_commit_if<false>(emmy::elect_one(), emmy::smem_u32(drain));
         volatile uint32_t never = 0u;
         emmy::mbar_wait(drain, 0u, &never, 0u, 20000000ull);
+        __syncwarp();
     }
     emmy::tc_fence_before();
     __syncthreads();
@@ -890,40 +917,38 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {
+        if (rank == 0) {
             // ---------------- MMA issuer (leader only)
             const Issue<I8, LAYOUT, true> issue(sA, sB, bf16, BN);
-            const uint32_t peer_empty = emmy::mapa(&empty[0], 1), peer_tfull = emmy::mapa(&tfull[0], 1);
             uint32_t stage = 0, phase = 0, it = 0;
             bool ok = true;
             for (int t = pair; t < total && ok; t += npairs, ++it) {
                 const Tile w = tile(t);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
-                if (!emmy::mbar_wait_cluster(&tempty[acc], aphase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) break;
+                ok = __all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tempty[acc], aphase ^ 1u, abort_flag,
+                                                                     EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
+                if (!ok) break;
                 emmy::tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * BN;
-                for (int kb = 0; kb < w.kb1; ++kb) {
-                    if (!emmy::mbar_wait_cluster(&full[stage], phase, abort_flag, EMMY_STATUS_TIMEOUT_MMA, kWaitNs)) {
-                        ok = false;
-                        break;
-                    }
+                const int blocks = uniform(w.kb1), last_steps = uniform(last_block_steps(w, w.kb1, BK));
+                for (int i = 0; i < blocks; ++i) {
+                    ok = __all_sync(0xffffffffu, emmy::mbar_wait_cluster(&full[stage], phase, abort_flag,
+                                                                         EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
+                    if (!ok) break;
                     emmy::tc_fence_after();
-                    const int have = w.kend - kb * BK;
-                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, kb > 0, have < BK ? (have + 15) / 16 : 4);
-                    emmy::umma_commit_pair(emmy::smem_u32(&empty[stage]));
-                    emmy::umma_commit_pair(peer_empty + stage * 8u);
+                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, i > 0,
+                                LAYOUT == kMM && i == blocks - 1 ? last_steps : 4);
+                    issue.commit(&empty[stage]);
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                emmy::umma_commit_pair(emmy::smem_u32(&tfull[acc]));
-                emmy::umma_commit_pair(peer_tfull + acc * 8u);
+                issue.commit(&tfull[acc]);
             }
             // arrives on both CTAs once every pair MMA has finished
-            emmy::umma_commit_pair(emmy::smem_u32(drain));
-            emmy::umma_commit_pair(emmy::mapa(drain, 1));
+            issue.commit(drain);
         }
         __syncwarp();
     } else {
