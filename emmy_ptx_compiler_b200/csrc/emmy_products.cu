@@ -304,13 +304,13 @@ cudaLaunchAttribute early_start() {
     return attr;
 }
 
-using TcKernel = void (*)(Product, bool, CUtensorMap, CUtensorMap);
+using TcKernel = void (*)(Product, Flags, CUtensorMap, CUtensorMap);
 
 // What every variant's launch takes.
 struct Launch {
     const Call &call;
     const Product &p;
-    bool bf16;
+    Flags flags;
     const CUtensorMap &ta, &tb;
     int64_t clusters;
     int cluster;
@@ -330,7 +330,7 @@ int launch_clusters(const Launch &l, TcKernel kernel, std::atomic<uint64_t> &rea
     attrs[1].val.clusterDim = {static_cast<unsigned>(l.cluster), 1, 1};
     cfg.attrs = attrs;
     cfg.numAttrs = 2;
-    return launched(l.call, cudaLaunchKernelEx(&cfg, kernel, l.p, l.bf16, l.ta, l.tb));
+    return launched(l.call, cudaLaunchKernelEx(&cfg, kernel, l.p, l.flags, l.ta, l.tb));
 }
 
 template <bool I8, int LAYOUT, int BN, bool TMA>
@@ -387,7 +387,8 @@ int launch_product(const Call &call, Product p, bool bf16) {
     }
     p.a_end = end_of(a, esize);
     p.b_end = end_of(b, esize);
-    const bool tma = encode_tiled() && tma_ready(a, esize) && tma_ready(b, esize);
+    const Flags flags{bf16, encode_tiled() && tma_ready(a, esize), encode_tiled() && tma_ready(b, esize)};
+    const bool tma = flags.tma_a && flags.tma_b;
 
     // groups that can hold rows, and the rows of an even one
     const int64_t groups = p.experts < p.rows ? p.experts : (p.rows ? p.rows : 1);
@@ -407,17 +408,15 @@ int launch_product(const Call &call, Product p, bool bf16) {
     }
     if (most(kTileM, p.dw ? 64 : 16) > kMaxExtent)
         return report(EMMY_ERR_INVALID, "%s: an output of more than 2^31 tiles is not supported", call.name);
-    const int bn = pair ? pair : p.dw ? 128 : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
+    const int bn = pair ? pair : p.dw ? 128 : !tma ? (even <= 24 ? 32 : 128) : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
 
     CUtensorMap ta{}, tb{};
-    if (tma) {
-        const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                         : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-        if (!encode(&ta, a, type, esize, 3, bk, a_mn ? 64 : kTileM) ||
-            !encode(&tb, b, type, esize, 2, bk, p.dw ? 64 : pair ? pair / 2 : bn))
-            return report(EMMY_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", call.name);
-    }
+    const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if ((flags.tma_a && !encode(&ta, a, type, esize, 3, bk, a_mn ? 64 : kTileM)) ||
+        (flags.tma_b && !encode(&tb, b, type, esize, 2, bk, p.dw ? 64 : pair ? pair / 2 : bn)))
+        return report(EMMY_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", call.name);
     const int resident = pair ? kSms : kSms * (tma && bn <= 32 ? 2 : 1);
     int split = 1;
     if (!pair)
@@ -425,7 +424,7 @@ int launch_product(const Call &call, Product p, bool bf16) {
     const int cluster = pair ? 2 : split;
     int64_t clusters = pair ? most(2 * kTileM, pair) : most(kTileM, bn);
     if (clusters > resident / cluster) clusters = resident / cluster;
-    const Launch l{call, p, bf16, ta, tb, clusters, cluster};
+    const Launch l{call, p, flags, ta, tb, clusters, cluster};
     if constexpr (I8) {
         return launch_variant<true, kKK>(l, tma, pair, bn);
     } else {

@@ -110,11 +110,24 @@ __device__ __forceinline__ void fence_proxy_async() {
 __device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
-    return v;
+// 16 bytes from global to shared memory in the background, both aligned; one group for each commit.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but this thread's `N` latest groups have arrived.
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
+// The two halves of cluster_sync().
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Instruction descriptors: kind::f16 with either operand MN-major, and kind::i8 (s8 x s8 -> s32).
 __host__ __device__ constexpr uint32_t idesc_f16_major(uint32_t ab_fmt, uint32_t a_mn, uint32_t b_mn, uint32_t m,
@@ -134,6 +147,11 @@ constexpr int kTileM = 128;
 constexpr uint32_t kBlockBytes = 128;                  // one 128-byte swizzle row of k (or of m, c)
 constexpr uint32_t kPanel = 64 * kBlockBytes;          // 64 k x 64 m (or c) of an MN-major 16-bit operand
 constexpr uint32_t kStageA = kTileM * kBlockBytes;
+
+struct Flags {
+    bool bf16;            // 16-bit operands are bf16, else f16
+    bool tma_a, tma_b;    // TMA can load the operand
+};
 
 // The operands' layouts: which of them are contiguous along m (c) instead of along k.
 enum : int { kKK = 0, kMK = 1, kMM = 2 };  // kMM: dw
@@ -199,15 +217,24 @@ __device__ __forceinline__ int last_block_steps(const Tile &w, int kb1, int bk) 
 // in L2 from one to the next.
 constexpr int kSweep = 8;
 
-// Tile t of the launch (tm x col_tile; host code keeps the tiles within 31 bits).  `e` is a cursor:
-// tiles of one caller come in ascending order.  A cluster of `split` CTAs divides the sum.
+// Tile t of the launch (tm x col_tile; host code keeps the tiles within 31 bits), for a whole warp.
+// `e` is a cursor: tiles of one caller come in ascending order, and each step looks 32 experts
+// ahead.  A cluster of `split` CTAs divides the sum.
 __device__ __forceinline__ Tile tile_at(const Product &p, const Groups &g, int t, int mt, int &e, int tm, int col_tile,
                                         int bk, uint32_t rank, uint32_t split) {
-    while (t >= mt * g.tiles[e + 1]) ++e;
+    for (const int lane = threadIdx.x & 31;; e += 32) {
+        const int i = e + 1 + lane;
+        const uint32_t past = __ballot_sync(0xffffffffu, i > p.experts || t < mt * g.tiles[min(i, p.experts)]);
+        if (past) {
+            e += __ffs(past) - 1;
+            break;
+        }
+    }
     const int begin = g.row[e], count = g.row[e + 1] - begin;
-    const uint32_t r = t - mt * g.tiles[e], sweep_tiles = kSweep * (g.tiles[e + 1] - g.tiles[e]);
-    const uint32_t sweep = r / sweep_tiles, in = r - sweep * sweep_tiles, first = sweep * kSweep;
-    const uint32_t wide = min(static_cast<uint32_t>(kSweep), mt - first), ci = in / wide;
+    const uint32_t r = t - mt * g.tiles[e], ct = g.tiles[e + 1] - g.tiles[e];
+    const uint32_t sweep = ct == 1 ? r / kSweep : r / kSweep / ct, in = r - sweep * kSweep * ct, first = sweep * kSweep;
+    const uint32_t wide = min(static_cast<uint32_t>(kSweep), mt - first);
+    const uint32_t ci = ct == 1 ? 0 : wide == kSweep ? in / kSweep : in / wide;
     Tile o;
     o.e = e;
     o.begin = begin;
@@ -215,19 +242,19 @@ __device__ __forceinline__ Tile tile_at(const Product &p, const Groups &g, int t
     o.c0 = static_cast<int>(ci) * col_tile;
     o.cols = min(col_tile, (p.dw ? static_cast<int>(p.c) : count) - o.c0);
     o.kend = p.dw ? count : static_cast<int>(p.k);
-    const uint32_t nkb = o.kend / bk + (o.kend % bk != 0);
-    o.kb0 = static_cast<int>(nkb * rank / split);
-    o.kb1 = static_cast<int>(nkb * (rank + 1) / split);
+    const uint32_t nkb = static_cast<uint32_t>(o.kend + bk - 1) / bk;
+    // split is a power of two
+    o.kb0 = static_cast<int>(nkb * rank >> (31 - __clz(split)));
+    o.kb1 = static_cast<int>(nkb * (rank + 1) >> (31 - __clz(split)));
     return o;
 }
 
-// Operands that TMA cannot address (rows that start off a 16-byte boundary) are loaded in units of
-// 64 bytes of a row, as the five aligned 16-byte words that cover them; the bytes are shifted into
-// place in registers.  A word is read whole where it lies inside the operand, whichever of its
-// bytes are wanted; at the operand's two ends it is put together from its bytes.
-struct Unit {
-    uint4 w[5];
-};
+// Operands that TMA cannot address (rows that start off a 16-byte boundary): a block's 128 bytes of a
+// row lie within 9 aligned 16-byte words.  These come to a staging row in the background, and
+// each 16-byte chunk of the swizzled operand is then cut out of two neighbouring words.  A word is
+// read whole where it lies inside the operand, whichever of its bytes are wanted; at the
+// operand's two ends it is put together from its bytes.
+constexpr uint32_t kStagedRow = 144;
 
 __device__ __noinline__ uint4 load_edge_word(const uint8_t *at, const uint8_t *lo, const uint8_t *hi) {
     alignas(16) uint8_t v[16];
@@ -235,49 +262,60 @@ __device__ __noinline__ uint4 load_edge_word(const uint8_t *at, const uint8_t *l
     return *reinterpret_cast<const uint4 *>(v);
 }
 
-// `bytes` (at most 64, may be negative) of the unit at `src` are wanted.
-__device__ __forceinline__ void load_unit(Unit &u, const uint8_t *src, int64_t bytes, const uint8_t *lo,
-                                          const uint8_t *hi) {
-    const uint8_t *at = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(src) & ~uintptr_t(15));
-    const uint8_t *end = src + (bytes < 64 ? bytes : 64);
+// Rows of an operand's block: row r at `src` + r * `stride` bytes, of which `valid` bytes are wanted in
+// the first `rows` of them.
+struct Rows {
+    const uint8_t *src, *lo, *hi;
+    int64_t stride, valid, rows;
+};
+
+// Start the loads of N rows from `r0` on into `staged`; one warp.
+template <int N>
+__device__ __forceinline__ void stage_rows(const Rows &b, int r0, uint8_t *staged, int lane) {
+    const int valid = static_cast<int>(b.valid < 128 ? b.valid : 128);
+    const uint32_t to = emmy::smem_u32(staged);
     #pragma unroll
-    for (int i = 0; i < 5; ++i, at += 16) {
-        u.w[i] = make_uint4(0, 0, 0, 0);
-        if (bytes > 0 && at < end) {
-            if (at >= lo && at + 16 <= hi) u.w[i] = *reinterpret_cast<const uint4 *>(at);
-            else u.w[i] = load_edge_word(at, lo, hi);
-        }
+    for (int k = 0; k < (N * 9 + 31) / 32; ++k) {
+        const int i = lane + 32 * k, r = i / 9, j = i - 9 * r;
+        const uint8_t *row = b.src + (r0 + r) * b.stride;
+        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15u);
+        const uint8_t *at = row - off + 16 * j;
+        const bool want = i < N * 9 && r0 + r < b.rows && 16 * j < off + valid, whole = at >= b.lo && at + 16 <= b.hi;
+        if (want && whole) emmy::cp_async16(to + r * kStagedRow + 16 * j, at);
+        if (want && !whole) *reinterpret_cast<uint4 *>(staged + r * kStagedRow + 16 * j) = load_edge_word(at, b.lo, b.hi);
     }
 }
 
-// The first `keep` bytes of a word (any value; below 0 counts as 0).
-__device__ __forceinline__ uint32_t keep_bytes(uint32_t v, int64_t keep) {
-    return keep >= 4 ? v : keep <= 0 ? 0u : v & ((1u << (8 * static_cast<int>(keep))) - 1u);
+// The first `keep` bytes of a word (below 0 counts as 0).
+__device__ __forceinline__ uint32_t keep_bytes(uint32_t v, int keep) {
+    return keep >= 4 ? v : keep <= 0 ? 0u : v & ((1u << (8 * keep)) - 1u);
 }
 
-// Shift a unit into place and store its four 16-byte chunks, zeros behind `bytes`, into row `row` of a
-// swizzled panel; `half`: which 64 bytes of the 128-byte row.
-__device__ __forceinline__ void store_unit(const Unit &u, const uint8_t *src, int64_t bytes, uint8_t *panel, int row,
-                                           int half) {
-    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src)) & 15u, bits = (off & 3u) * 8u;
-    const uint32_t *w = reinterpret_cast<const uint32_t *>(&u);
-    uint32_t v[17];
+// Cut the staged rows into the swizzled 128-byte rows of `operand`, zeros where nothing is wanted; one
+// warp, the one that staged them.
+template <int N>
+__device__ __forceinline__ void cut_rows(const Rows &b, int r0, const uint8_t *staged, uint8_t *operand, int lane) {
+    const int valid = static_cast<int>(b.valid < 128 ? b.valid : 128), j = lane & 7;
+    const uint32_t low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(b.src)), low_stride = static_cast<uint32_t>(b.stride);
     #pragma unroll
-    for (int i = 0; i < 17; ++i) {
-        // word off / 4 + i of the 20, without indexing registers by a variable
-        const uint32_t near = off & 4u ? w[i + 1] : w[i], far = off & 4u ? w[i + 3] : w[i + 2];
-        v[i] = off & 8u ? far : near;
-    }
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t c[4];
+    for (int k = 0; k < N / 4; ++k) {
+        const int r = (lane >> 3) + 4 * k, row = r0 + r, have = row < b.rows ? valid - 16 * j : 0;
+        const uint32_t off = low + row * low_stride;  // its low 4 bits count
+        const uint4 *w = reinterpret_cast<const uint4 *>(staged + r * kStagedRow + 16 * j);
+        const uint4 w0 = w[0], w1 = w[1];
+        const uint32_t a[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        uint32_t h[6], v[5], c[4];
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            c[i] = __funnelshift_r(v[4 * j + i], v[4 * j + i + 1], bits);
-            if (bytes < 64) c[i] = keep_bytes(c[i], bytes - 16 * j - 4 * i);
+        for (int q = 0; q < 6; ++q) h[q] = off & 8u ? a[q + 2] : a[q];
+        #pragma unroll
+        for (int q = 0; q < 5; ++q) v[q] = off & 4u ? h[q + 1] : h[q];
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) c[q] = __funnelshift_r(v[q], v[q + 1], (off & 3u) * 8u);
+        if (have < 16) {
+            #pragma unroll
+            for (int q = 0; q < 4; ++q) c[q] = keep_bytes(c[q], have - 4 * q);
         }
-        *reinterpret_cast<uint4 *>(panel + row * kBlockBytes + (((half * 4 + j) ^ (row & 7)) << 4)) =
-            make_uint4(c[0], c[1], c[2], c[3]);
+        *reinterpret_cast<uint4 *>(operand + row * kBlockBytes + ((j ^ (row & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
     }
 }
 
@@ -297,18 +335,39 @@ __device__ __forceinline__ int64_t out_index(const Product &p, const Tile &t, in
     return (p.dw ? t.e * p.out_e : t.begin * p.out_c) + (t.c0 + static_cast<int64_t>(c)) * p.out_c + m;
 }
 
-// Scale of a channel, and its bias.
+// Scale of a channel, and its bias; loaded before the sums are ready.
 struct Channel {
     float scale = 0.0f, bias = 0.0f;
 };
+template <bool I8>
 __device__ __forceinline__ Channel channel(const Product &p, const Tile &t, int64_t m) {
     Channel c;
-    if (m < p.m) {
+    if (I8 && m < p.m) {
         c.scale = p.w_scale[t.e * p.m + m];
         if (p.bias) c.bias = p.bias[t.e * p.m + m];
     }
     return c;
 }
+
+// Scales of N x 32 output rows from `from` on, lane l holding those of rows 32 i + l.
+template <bool I8, int N>
+struct RowScales {
+    float v[N];
+    __device__ __forceinline__ RowScales(const Product &p, const Tile &t, int from, int lane) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = from + 32 * i + lane;
+            v[i] = I8 && c < t.cols ? p.x_scale[t.begin + t.c0 + c] : 0.0f;
+        }
+    }
+    // of row `i` of the first 32
+    __device__ __forceinline__ float at(int i) const { return I8 ? __shfl_sync(0xffffffffu, v[0], i) : 0.0f; }
+    __device__ __forceinline__ void next() {
+        #pragma unroll
+        for (int i = 0; i + 1 < N; ++i) v[i] = v[i + 1];
+    }
+};
+
 template <bool I8>
 __device__ __forceinline__ float scaled(uint32_t bits, float row_scale, const Channel &c) {
     if constexpr (I8) return sum_value<true>(bits) * row_scale * c.scale + c.bias;
@@ -333,22 +392,17 @@ __device__ __forceinline__ uint32_t pack16(bool bf16, float lo, float hi) {
 // go to shared memory through stmatrix, and 4 lanes then write each 64-byte piece of an output row
 // 16 bytes at a time (4 stores for 32 rows instead of 32, and the conversion packs two values).  f32
 // outputs need no help: 32 lanes write 128 bytes of a row.  `empty`: the sum had no terms.
-template <bool I8>
+template <bool I8, int N>
 __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int mq, uint32_t taddr, bool empty, int from,
-                                           int to, uint8_t *buf, int lane) {
-    if (to > w.cols) to = w.cols;
-    if (from >= to) return;
+                                           const Channel &own, RowScales<I8, N> xs, uint8_t *buf, int lane) {
+    const int to = min(from + 32 * N, w.cols);
     if (p.out_type == EMMY_F32) {
         const int64_t m = mq + lane;
-        Channel ch;
-        if constexpr (I8) ch = channel(p, w, m);
         float *out = static_cast<float *>(p.out) + out_index(p, w, m, from);
         #pragma unroll 1
-        for (int c = from; c < to; c += 32, out += 32 * p.out_c) {
+        for (int c = from; c < to; c += 32, out += 32 * p.out_c, xs.next()) {
             uint32_t r[32];
             emmy::tmem_ld_32x32b_x32(taddr + c, r);
-            float xs = 0.0f;
-            if (I8 && c + lane < to) xs = p.x_scale[w.begin + w.c0 + c + lane];
             emmy::tmem_ld_wait();
             if (empty) {
                 #pragma unroll
@@ -357,7 +411,7 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
             float *o = out;
             #pragma unroll
             for (int j = 0; j < 32; ++j, o += p.out_c) {
-                const float v = scaled<I8>(r[j], I8 ? __shfl_sync(0xffffffffu, xs, j) : 0.0f, ch);
+                const float v = scaled<I8>(r[j], xs.at(j), own);
                 if (m < p.m && c + j < to) *o = v;
             }
         }
@@ -370,21 +424,19 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
     Channel ch[4];
     if constexpr (I8) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) ch[i] = channel(p, w, mq + lane / 4 + 8 * i);
+        for (int i = 0; i < 4; ++i) {
+            ch[i].scale = __shfl_sync(0xffffffffu, own.scale, lane / 4 + 8 * i);
+            ch[i].bias = __shfl_sync(0xffffffffu, own.bias, lane / 4 + 8 * i);
+        }
     }
     #pragma unroll 1
-    for (int c = from; c < to; c += 32, out += 32 * p.out_c) {
+    for (int c = from; c < to; c += 32, out += 32 * p.out_c, xs.next()) {
         uint32_t r[2][16];
         emmy::tmem_ld_16x256b_x4(taddr + c, r[0]);
         emmy::tmem_ld_16x256b_x4(taddr + (16u << 16) + c, r[1]);
-        float xs[8];
-        if constexpr (I8) {
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int col = c + 8 * (i >> 1) + 2 * piece + (i & 1);
-                xs[i] = col < to ? p.x_scale[w.begin + w.c0 + col] : 0.0f;
-            }
-        }
+        float x[8];
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = xs.at(8 * (i >> 1) + 2 * piece + (i & 1));
         emmy::tmem_ld_wait();
         if (empty) {
             #pragma unroll
@@ -396,8 +448,7 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
             #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int row = 2 * h + (i & 1), col = i >> 1 << 1;
-                v[i] = pack16(bf16, scaled<I8>(r[h][2 * i], I8 ? xs[col] : 0.0f, ch[row]),
-                              scaled<I8>(r[h][2 * i + 1], I8 ? xs[col + 1] : 0.0f, ch[row]));
+                v[i] = pack16(bf16, scaled<I8>(r[h][2 * i], x[col], ch[row]), scaled<I8>(r[h][2 * i + 1], x[col + 1], ch[row]));
             }
             const uint32_t at = emmy::smem_u32(buf) + ((lane >> 4) * 8 + (lane & 7)) * kStoreRow +
                                 (16 * h + 8 * ((lane >> 3) & 1)) * 2;
@@ -421,27 +472,46 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
     }
 }
 
+// Send 16 columns' sums from `c` on, for one channel, to the CTAs that finish them: 16 / G columns to
+// each of G.  `own`: this rank's place in a CTA's exchange buffer, in bytes.
+template <int G>
+__device__ __forceinline__ void send_columns(const uint32_t *red, uint32_t own, uint32_t share, int share_log, int c,
+                                             int cols, const uint32_t (&r)[16], bool none) {
+    #pragma unroll
+    for (int d = 0; d < G; ++d) {
+        const int first = c + d * (16 / G);
+        if (first >= cols) break;
+        const uint32_t at = emmy::mapa(red, first >> share_log) + own + (first & (share - 1)) * kTileM * 4;
+        #pragma unroll
+        for (int j = 0; j < 16 / G; ++j)
+            if (first + j < cols) emmy::st_cluster_u32(at + j * kTileM * 4, none ? 0u : r[d * (16 / G) + j]);
+    }
+}
+
 template <bool I8, int BN, bool TMA>
 struct TcConfig {
     static constexpr uint32_t kStageB = BN * kBlockBytes;
     static constexpr uint32_t kStage = kStageA + kStageB;
     static constexpr uint32_t kRed = BN * kTileM * 4;  // partial sums for the cluster
-    static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
-    static constexpr int kOut = BN >= 64 ? 8 : 4;  // warps that turn sums into output
-    static constexpr int kLoaders = TMA ? 1 : 8;   // warps that fill the stages
-    static constexpr int kThreads = 64 + 32 * kOut + (TMA ? 0 : 32 * kLoaders);
-    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + 256;
+    static constexpr int kStages = !TMA ? (BN == 32 ? 3 : 2) : BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
+    static constexpr int kStaged = !TMA ? (BN == 32 ? 4 : 2) : 0;  // blocks on their way to be cut into place
+    static constexpr uint32_t kStagedBytes = (kTileM + BN) * kStagedRow;
+    static constexpr int kOut = BN >= 64 && TMA ? 8 : 4;  // warps that turn sums into output
+    static constexpr int kLoaders = TMA ? 0 : 8;  // warps that load without TMA
+    static constexpr int kThreads = 64 + 32 * (kOut + kLoaders);
+    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + kStaged * kStagedBytes + 256;
+    static constexpr int kPerSm = TMA && BN <= 32 ? 2 : 1;  // CTAs that share an SM
     static constexpr uint32_t kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
-// Warp 0 loads operand tiles by TMA (TMA false: the last 8 warps do, with plain loads, for
-// rows TMA cannot take), warp 1 issues the MMAs into one of two accumulators, the warps from 2 on
+// Warp 0 loads operand tiles by TMA (TMA false: the last 8 warps load those operands whose rows
+// TMA cannot take), warp 1 issues the MMAs into one of two accumulators, the warps from 2 on
 // turn the other into output, 4 or 8 of them: a warp reaches 32 of the 128 lanes.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
-// added in rank order through distributed shared memory, each CTA finishing its share of columns:
-// the result depends on neither timing nor the number of SMs.
+// added in rank order: each CTA finishes its share of the columns, for which the others send their
+// parts through distributed shared memory.  The result depends on neither timing nor the number of SMs.
 template <bool I8, int LAYOUT, int BN, bool TMA>
-__global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
-    product_tc_kernel(const Product p, const bool bf16, const __grid_constant__ CUtensorMap tm_a,
+__global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, BN, TMA>::kPerSm)
+    product_tc_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
                       const __grid_constant__ CUtensorMap tm_b) {
     using Cfg = TcConfig<I8, BN, TMA>;
     using T = std::conditional_t<I8, int8_t, uint16_t>;
@@ -454,7 +524,8 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
     uint8_t *sA = smem;
     uint8_t *sB = sA + STAGES * kStageA;
     uint32_t *red = reinterpret_cast<uint32_t *>(sB + STAGES * Cfg::kStageB);
-    uint64_t *full = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(red) + Cfg::kRed);
+    uint8_t *staged = reinterpret_cast<uint8_t *>(red) + Cfg::kRed;
+    uint64_t *full = reinterpret_cast<uint64_t *>(staged + Cfg::kStaged * Cfg::kStagedBytes);
     uint64_t *empty = full + STAGES;
     uint64_t *tfull = empty + STAGES;
     uint64_t *tempty = tfull + 2;
@@ -466,7 +537,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
 
     if (threadIdx.x == 64) {
         for (int s = 0; s < STAGES; ++s) {
-            emmy::mbar_init(&full[s], Cfg::kLoaders);
+            emmy::mbar_init(&full[s], 1 + Cfg::kLoaders);
             emmy::mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -482,9 +553,9 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
         emmy::tmem_relinquish();
     }
     if (warp == 0) {
-        if (TMA && lane == 0) {
-            emmy::tma_prefetch(&tm_a);
-            emmy::tma_prefetch(&tm_b);
+        if (lane == 0) {
+            if (TMA || flags.tma_a) emmy::tma_prefetch(&tm_a);
+            if (TMA || flags.tma_b) emmy::tma_prefetch(&tm_b);
         }
     }
     emmy::wait_for_prior_grid();
@@ -494,42 +565,47 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
     emmy::tc_fence_after();
     emmy::let_next_grid_start();
     const uint32_t tmem_base = *tmem_holder;
+    bool met = split == 1;  // the cluster's other CTAs have started: their shared memory may be written
+    if (!met) emmy::cluster_arrive();
 
     const int mt = static_cast<int>((p.m + kTileM - 1) / kTileM), total = mt * g.tiles[p.experts];
     const int step = static_cast<int>(gridDim.x / split);
     uint32_t stage = 0, phase = 0, it = 0;
     uint32_t issued = 0u, parity_bits = 0u;  // producer: loads in flight for each stage and their parity
     bool ok = true;
+    const uint32_t share = BN / split, share_log = 31 - __clz(share);  // columns of a tile that each CTA finishes
     int e = 0;
     // Without a cluster each role runs through all of the CTA's tiles at its own pace; a cluster
     // takes one tile at a time, because its CTAs meet after each.
     for (int first = static_cast<int>(blockIdx.x / split); first < total; first += split > 1 ? step : total) {
         const int last = split > 1 ? first + 1 : total;
-        if (TMA && warp == 0) {
-            if (lane == 0) {
-                for (int t = first; t < last && ok; t += step) {
-                    const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
+        if (warp == 0) {
+            const bool ta = TMA || flags.tma_a, tb = TMA || flags.tma_b;
+            const uint32_t bytes = (ta ? kStageA : 0) + (tb ? Cfg::kStageB : 0);
+            for (int t = first; t < last && ok; t += step) {
+                const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
+                if (lane == 0) {
                     for (int kb = w.kb0; kb < w.kb1; ++kb) {
                         if (!emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
                             ok = false;
                             break;
                         }
-                        emmy::mbar_arrive_expect_tx(&full[stage], Cfg::kStage);
+                        emmy::mbar_arrive_expect_tx(&full[stage], bytes);
                         uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
                         const int k0 = kb * BK;
                         if constexpr (LAYOUT == kKK) {
-                            emmy::tma_load_3d(a, &tm_a, &full[stage], k0, w.m0, w.e);
-                        } else {
+                            if (ta) emmy::tma_load_3d(a, &tm_a, &full[stage], k0, w.m0, w.e);
+                        } else if (ta) {
                             const int ka = LAYOUT == kMM ? w.begin + k0 : k0, ez = LAYOUT == kMM ? 0 : w.e;
                             emmy::tma_load_3d(a, &tm_a, &full[stage], w.m0, ka, ez);
                             emmy::tma_load_3d(a + kPanel, &tm_a, &full[stage], w.m0 + 64, ka, ez);
                         }
-                        if constexpr (LAYOUT == kMM) {
+                        if constexpr (LAYOUT != kMM) {
+                            if (tb) emmy::tma_load_2d(b, &tm_b, &full[stage], k0, w.begin + w.c0);
+                        } else if (tb) {
                             #pragma unroll
                             for (int j = 0; j < BN / 64; ++j)
                                 emmy::tma_load_2d(b + j * kPanel, &tm_b, &full[stage], w.c0 + 64 * j, w.begin + k0);
-                        } else {
-                            emmy::tma_load_2d(b, &tm_b, &full[stage], k0, w.begin + w.c0);
                         }
                         issued |= 1u << stage;
                         parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
@@ -539,58 +615,71 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                         }
                     }
                 }
+                ok = __all_sync(0xffffffffu, ok);
             }
-            __syncwarp();
         } else if (!TMA && warp >= 2 + Cfg::kOut) {
-            // 256 threads: one unit of A (128 rows x 2 halves) and at most one of B each, the next
-            // block's loads in flight while this block's are stored
-            const int th = threadIdx.x - 64 - 32 * Cfg::kOut, half = th & 1;
-            const uint8_t *a_lo = static_cast<const uint8_t *>(p.a), *a_hi = static_cast<const uint8_t *>(p.a_end);
-            const uint8_t *b_lo = static_cast<const uint8_t *>(p.b), *b_hi = static_cast<const uint8_t *>(p.b_end);
-            const bool has_b = th < 2 * BN;
+            // Each of the 8 warps has 16 rows of A and BN / 8 of B to itself: it stages and cuts them
+            // without waiting for the others.  Rows run along m (c), or along k in panels of 64.
+            const int lw = warp - 2 - Cfg::kOut, slot0 = lw * 16, slotb0 = lw * (BN / 8);
+            const bool has_a = !flags.tma_a, has_b = !flags.tma_b;
+            constexpr int DEPTH = TMA ? 1 : Cfg::kStaged;
+            constexpr int64_t ES = sizeof(T);
             for (int t = first; t < last && ok; t += step) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const T *ae = static_cast<const T *>(p.a) + (p.dw ? w.begin * p.a_k : w.e * p.a_e);
                 const T *be = static_cast<const T *>(p.b) + w.begin * (p.dw ? p.b_k : p.b_c);
-                Unit ua, ub;
-                const uint8_t *pa = nullptr, *pb = nullptr;
-                int64_t na = 0, nb = 0;
-                // where this thread's units of block kb lie, and how many of their bytes are wanted
-                auto load = [&](int kb) {
+                auto rows_a = [&](int kb) {
                     const int64_t k0 = static_cast<int64_t>(kb) * BK, kleft = w.kend - k0;
-                    const int64_t row = th >> 1, krow = row & 63, panel = row >> 6;
-                    if constexpr (LAYOUT != kKK) {
-                        const int64_t m = w.m0 + 64 * panel;
-                        pa = reinterpret_cast<const uint8_t *>(ae + (k0 + krow) * p.a_k + m);
-                        na = krow < kleft ? (p.m - m) * static_cast<int64_t>(sizeof(T)) : 0;
+                    Rows r;
+                    r.lo = static_cast<const uint8_t *>(p.a);
+                    r.hi = static_cast<const uint8_t *>(p.a_end);
+                    if constexpr (LAYOUT == kKK) {
+                        r.src = reinterpret_cast<const uint8_t *>(ae + w.m0 * p.a_m + k0);
+                        r.stride = p.a_m * ES, r.valid = kleft * ES, r.rows = p.m - w.m0;
                     } else {
-                        pa = reinterpret_cast<const uint8_t *>(ae + (w.m0 + row) * p.a_m + k0);
-                        na = row < p.m - w.m0 ? kleft * static_cast<int64_t>(sizeof(T)) : 0;
+                        // this warp's 16 rows lie in one panel
+                        const int64_t m = w.m0 + (slot0 & 64);
+                        r.src = reinterpret_cast<const uint8_t *>(ae + (k0 - (slot0 & 64)) * p.a_k + m);
+                        r.stride = p.a_k * ES, r.valid = (p.m - m) * ES, r.rows = kleft + (slot0 & 64);
                     }
-                    pa += 64 * half;
-                    na -= 64 * half;
-                    load_unit(ua, pa, na, a_lo, a_hi);
-                    if (!has_b) return;
-                    if constexpr (LAYOUT == kMM) {
-                        pb = reinterpret_cast<const uint8_t *>(be + (k0 + krow) * p.b_k + w.c0 + 64 * panel);
-                        nb = krow < kleft ? (w.cols - 64 * panel) * static_cast<int64_t>(sizeof(T)) : 0;
-                    } else {
-                        pb = reinterpret_cast<const uint8_t *>(be + (w.c0 + row) * p.b_c + k0);
-                        nb = row < w.cols ? kleft * static_cast<int64_t>(sizeof(T)) : 0;
-                    }
-                    pb += 64 * half;
-                    nb -= 64 * half;
-                    load_unit(ub, pb, nb, b_lo, b_hi);
+                    return r;
                 };
-                if (w.kb0 < w.kb1) load(w.kb0);
-                for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    if (!emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
-                        ok = false;
-                        break;
+                auto rows_b = [&](int kb) {
+                    const int64_t k0 = static_cast<int64_t>(kb) * BK, kleft = w.kend - k0;
+                    Rows r;
+                    r.lo = static_cast<const uint8_t *>(p.b);
+                    r.hi = static_cast<const uint8_t *>(p.b_end);
+                    if constexpr (LAYOUT != kMM) {
+                        r.src = reinterpret_cast<const uint8_t *>(be + w.c0 * p.b_c + k0);
+                        r.stride = p.b_c * ES, r.valid = kleft * ES, r.rows = w.cols;
+                    } else {
+                        const int64_t c = slotb0 & 64;
+                        r.src = reinterpret_cast<const uint8_t *>(be + (k0 - c) * p.b_k + w.c0 + c);
+                        r.stride = p.b_k * ES, r.valid = (w.cols - c) * ES, r.rows = kleft + c;
                     }
-                    // a 128-row K-major tile and two 64-row panels are laid out alike
-                    store_unit(ua, pa, na, sA + stage * kStageA, th >> 1, half);
-                    if (has_b) store_unit(ub, pb, nb, sB + stage * Cfg::kStageB, th >> 1, half);
+                    return r;
+                };
+                auto staging = [&](int kb) { return staged + kb % DEPTH * Cfg::kStagedBytes; };
+                auto stage_block = [&](int kb) {
+                    if (kb < w.kb1) {
+                        if (has_a) stage_rows<16>(rows_a(kb), slot0, staging(kb) + slot0 * kStagedRow, lane);
+                        if (has_b)
+                            stage_rows<BN / 8>(rows_b(kb), slotb0, staging(kb) + (kTileM + slotb0) * kStagedRow, lane);
+                    }
+                    emmy::cp_async_commit();
+                };
+                for (int i = 0; i < DEPTH; ++i) stage_block(w.kb0 + i);
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    emmy::cp_async_wait<DEPTH - 1>();
+                    ok = __all_sync(0xffffffffu, emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag,
+                                                                 EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs));
+                    if (!ok) break;
+                    __syncwarp();  // what the other lanes loaded is here too
+                    if (has_a)
+                        cut_rows<16>(rows_a(kb), slot0, staging(kb) + slot0 * kStagedRow, sA + stage * kStageA, lane);
+                    if (has_b)
+                        cut_rows<BN / 8>(rows_b(kb), slotb0, staging(kb) + (kTileM + slotb0) * kStagedRow,
+                                 sB + stage * Cfg::kStageB, lane);
                     emmy::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) emmy::mbar_arrive(&full[stage]);
@@ -598,11 +687,13 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                         stage = 0;
                         phase ^= 1u;
                     }
-                    if (kb + 1 < w.kb1) load(kb + 1);
+                    stage_block(kb + DEPTH);
                 }
+                emmy::cp_async_wait<0>();
+                __syncwarp();
             }
         } else if (warp == 1) {
-            const Issue<I8, LAYOUT, false> issue(sA, sB, bf16, BN);
+            const Issue<I8, LAYOUT, false> issue(sA, sB, flags.bf16, BN);
             for (int t = first; t < last && ok; t += step, ++it) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
@@ -617,7 +708,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
                                                                  EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
                     if (!ok) break;
                     const int steps = LAYOUT == kMM && i == blocks - 1 ? last_steps : 4;
-                    if (LAYOUT == kMM && TMA && i == blocks - 1) {
+                    if (LAYOUT == kMM && i == blocks - 1) {
                         // a block that ends inside: later rows belong to the next group (or hold
                         // anything), so what the last MMA takes of them becomes zero in both operands
                         const int have = min(BK, w.kend - (w.kb1 - 1) * BK);
@@ -643,40 +734,47 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
             __syncwarp();
         } else if (warp >= 2 && warp < 2 + Cfg::kOut) {
             const int q = warp & 3, part = (warp - 2) >> 2;
-            constexpr int PARTS = Cfg::kOut / 4, SPAN = BN / PARTS;
+            constexpr int SPAN = BN / (Cfg::kOut / 4);
             for (int t = first; t < last && ok; t += step, ++it) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
-                if (!emmy::mbar_wait(&tfull[acc], aphase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)) {
-                    ok = false;
-                    break;
-                }
+                const int64_t m = w.m0 + q * 32 + lane;
+                const Channel ch = channel<I8>(p, w, m);
+                RowScales<I8, (SPAN + 31) / 32> xs(p, w, part * SPAN, lane);
+                ok = __all_sync(0xffffffffu, emmy::mbar_wait(&tfull[acc], aphase, abort_flag,
+                                                             EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs));
+                if (!ok) break;
                 emmy::tc_fence_after();
                 const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
                 const bool none = w.kb0 == w.kb1;  // nothing was accumulated
                 if (BN >= 64 && split == 1) {
                     // the sums' exchange buffer is free without a cluster
-                    store_tile<I8>(p, w, w.m0 + q * 32, taddr, none, part * SPAN, (part + 1) * SPAN,
+                    store_tile<I8>(p, w, w.m0 + q * 32, taddr, none, part * SPAN, ch, xs,
                                    reinterpret_cast<uint8_t *>(red) + (warp - 2) * kStoreBytes, lane);
                 } else {
                     // few columns, or parts of sums: channels of a column are neighbours either way
-                    const int64_t m = w.m0 + q * 32 + lane;
-                    Channel ch;
-                    if (I8 && split == 1) ch = channel(p, w, m);
+                    if (!met) {
+                        emmy::cluster_wait();
+                        met = true;
+                    }
+                    const uint32_t own = (rank * share * kTileM + q * 32 + lane) * 4;
                     #pragma unroll 1
                     for (int c = part * SPAN; c < min((part + 1) * SPAN, w.cols); c += 16) {
                         uint32_t r[16];
                         emmy::tmem_ld_32x32b_x16(taddr + c, r);
                         emmy::tmem_ld_wait();
-                        #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            if (c + j >= w.cols) break;
-                            const uint32_t v = none ? 0u : r[j];
-                            if (split > 1)
-                                red[(c + j) * kTileM + q * 32 + lane] = v;
-                            else if (m < p.m)
-                                store_out(p.out, p.out_type, out_index(p, w, m, c + j),
-                                          scaled<I8>(v, I8 ? p.x_scale[w.begin + w.c0 + c + j] : 0.0f, ch));
+                        if (split > 1) {
+                            if (share >= 16) send_columns<1>(red, own, share, share_log, c, w.cols, r, none);
+                            else if (share == 8) send_columns<2>(red, own, share, share_log, c, w.cols, r, none);
+                            else if (share == 4) send_columns<4>(red, own, share, share_log, c, w.cols, r, none);
+                            else send_columns<8>(red, own, share, share_log, c, w.cols, r, none);
+                        } else {
+                            #pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const float v = scaled<I8>(none ? 0u : r[j], xs.at((c & 16) + j), ch);
+                                if (m < p.m && c + j < w.cols)
+                                    store_out(p.out, p.out_type, out_index(p, w, m, c + j), v);
+                            }
                         }
                     }
                 }
@@ -686,32 +784,54 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, 1)
             }
         }
         if (split > 1) {
-            __syncwarp();
-            emmy::cluster_sync();  // every CTA's partial sums are in its shared memory
-            if (warp >= 2 && warp < 2 + Cfg::kOut && ok) {
-                const Tile w = tile_at(p, g, first, mt, e, kTileM, BN, BK, rank, split);
-                const int lm = (warp & 3) * 32 + lane, part = (warp - 2) >> 2, parts = Cfg::kOut / 4;
-                const int64_t m = w.m0 + lm;
-                if (m < p.m) {
-                    Channel ch;
-                    if constexpr (I8) ch = channel(p, w, m);
-                    for (int c = rank + split * part; c < w.cols; c += split * parts) {
-                        uint32_t sum = 0u;  // 0 of either type
-                        for (uint32_t s = 0; s < split; ++s) {
-                            const uint32_t v = emmy::ld_cluster_u32(emmy::mapa(&red[c * kTileM + lm], s));
-                            sum = I8 ? sum + v : __float_as_uint(__uint_as_float(sum) + __uint_as_float(v));
-                        }
-                        store_out(p.out, p.out_type, out_index(p, w, m, c),
-                                  scaled<I8>(sum, I8 ? p.x_scale[w.begin + w.c0 + c] : 0.0f, ch));
-                    }
-                }
+            // the columns that this CTA finishes, their scales loaded before the parts arrive
+            const bool out_warp = warp >= 2 && warp < 2 + Cfg::kOut && ok;
+            const int lm = (warp & 3) * 32 + lane, part = (warp - 2) >> 2, parts = Cfg::kOut / 4;
+            const int from = static_cast<int>(rank * share);
+            Tile w{};
+            Channel ch;
+            float xs = 0.0f;
+            if (out_warp) {
+                w = tile_at(p, g, first, mt, e, kTileM, BN, BK, rank, split);
+                ch = channel<I8>(p, w, w.m0 + lm);
+                if (I8 && from + lane < w.cols) xs = p.x_scale[w.begin + w.c0 + from + lane];
             }
             __syncwarp();
-            emmy::cluster_sync();  // and may be overwritten
+            if (!met) {
+                emmy::cluster_wait();
+                met = true;
+            }
+            emmy::cluster_sync();  // this CTA's columns have arrived from every rank
+            if (out_warp) {
+                const int64_t m = w.m0 + lm;
+                const int to = min(from + static_cast<int>(share), w.cols);
+                #pragma unroll 4
+                for (int c = from + part; c < to; c += parts) {
+                    const uint32_t *at = red + (c - from) * kTileM + lm;
+                    uint32_t v[8], sum = 0u;  // 0 of either type
+                    #pragma unroll
+                    for (int s = 0; s < 8; ++s) v[s] = s < split ? at[s * share * kTileM] : 0u;
+                    #pragma unroll
+                    for (int s = 0; s < 8; ++s)
+                        if (s < split)
+                            sum = I8 ? sum + v[s] : __float_as_uint(__uint_as_float(sum) + __uint_as_float(v[s]));
+                    float x = 0.0f;
+                    if constexpr (I8) x = c - from < 32 ? __shfl_sync(0xffffffffu, xs, c - from) : p.x_scale[w.begin + w.c0 + c];
+                    if (m < p.m) store_out(p.out, p.out_type, out_index(p, w, m, c), scaled<I8>(sum, x, ch));
+                }
+            }
+            if (first + step < total) {
+                __syncwarp();
+                emmy::cluster_sync();  // and may be overwritten
+            }
         }
     }
+    if (!met) {
+        __syncwarp();
+        emmy::cluster_wait();
+    }
 
-    if (TMA && warp == 0 && lane == 0 && !ok) {
+    if (warp == 0 && lane == 0 && !ok) {
         // this CTA's own loads still in flight land before it leaves (bounded)
         volatile uint32_t never = 0u;
         for (int s = 0; s < STAGES; ++s)
@@ -753,7 +873,7 @@ struct PairConfig {
 
 template <bool I8, int LAYOUT, int BN>
 __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
-    product_pair_kernel(const Product p, const bool bf16, const __grid_constant__ CUtensorMap tm_a,
+    product_pair_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
                         const __grid_constant__ CUtensorMap tm_b) {
     using Cfg = PairConfig<BN>;
     constexpr int STAGES = Cfg::kStages, BK = I8 ? 128 : 64, CN = BN / 2;
@@ -869,11 +989,11 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
                     next();
                 }
             }
+            ok = __all_sync(0xffffffffu, ok);
             if constexpr (LAYOUT == kMM) {
                 // A last block that ends inside: later rows belong to the next group (or hold
                 // anything), and what the last MMA takes of them becomes zero in both operands
                 // before the leader's barrier completes.  The whole warp does that.
-                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 stage = __shfl_sync(0xffffffffu, stage, 0);
                 phase = __shfl_sync(0xffffffffu, phase, 0);
@@ -919,7 +1039,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
     } else if (warp == 1) {
         if (rank == 0) {
             // ---------------- MMA issuer (leader only)
-            const Issue<I8, LAYOUT, true> issue(sA, sB, bf16, BN);
+            const Issue<I8, LAYOUT, true> issue(sA, sB, flags.bf16, BN);
             uint32_t stage = 0, phase = 0, it = 0;
             bool ok = true;
             for (int t = pair; t < total && ok; t += npairs, ++it) {
@@ -960,10 +1080,14 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
         for (int t = pair; t < total; t += npairs, ++it) {
             const Tile w = tile(t);
             const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
-            if (!emmy::mbar_wait_cluster(&tfull[acc], aphase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)) break;
+            const Channel ch = channel<I8>(p, w, w.m0 + q * 32 + lane);
+            const RowScales<I8, SPAN / 32> xs(p, w, part * SPAN, lane);
+            if (!__all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tfull[acc], aphase, abort_flag,
+                                                                 EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)))
+                break;
             emmy::tc_fence_after();
             store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
-                           part * SPAN, (part + 1) * SPAN, sStore + (warp - 2) * kStoreBytes, lane);
+                           part * SPAN, ch, xs, sStore + (warp - 2) * kStoreBytes, lane);
             emmy::tc_fence_before();
             __syncwarp();
             if (lane == 0) emmy::mbar_arrive_cluster(leader_tempty + acc * 8u);
