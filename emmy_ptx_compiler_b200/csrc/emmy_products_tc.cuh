@@ -110,17 +110,6 @@ __device__ __forceinline__ void fence_proxy_async() {
 __device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// 16 bytes from global to shared memory in the background, both aligned; one group for each commit.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but this thread's `N` latest groups have arrived.
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
@@ -249,13 +238,10 @@ __device__ __forceinline__ Tile tile_at(const Product &p, const Groups &g, int t
     return o;
 }
 
-// Operands that TMA cannot address (rows that start off a 16-byte boundary): a block's 128 bytes of a
-// row lie within 9 aligned 16-byte words.  These come to a staging row in the background, and
-// each 16-byte chunk of the swizzled operand is then cut out of two neighbouring words.  A word is
-// read whole where it lies inside the operand, whichever of its bytes are wanted; at the
-// operand's two ends it is put together from its bytes.
-constexpr uint32_t kStagedRow = 144;
-
+// Operands that TMA cannot address (rows that start off a 16-byte boundary): each 16-byte chunk of the
+// swizzled operand is cut out of the two aligned 16-byte words that it lies in.  A word is read
+// whole where it lies inside the operand, whichever of its bytes are wanted; at the operand's two
+// ends it is put together from its bytes.
 __device__ __noinline__ uint4 load_edge_word(const uint8_t *at, const uint8_t *lo, const uint8_t *hi) {
     alignas(16) uint8_t v[16];
     for (int i = 0; i < 16; ++i) v[i] = at + i >= lo && at + i < hi ? at[i] : 0;
@@ -269,51 +255,64 @@ struct Rows {
     int64_t stride, valid, rows;
 };
 
-// Start the loads of N rows from `r0` on into `staged`; one warp.
-template <int N>
-__device__ __forceinline__ void stage_rows(const Rows &b, int r0, uint8_t *staged, int lane) {
-    const int valid = static_cast<int>(b.valid < 128 ? b.valid : 128);
-    const uint32_t to = emmy::smem_u32(staged);
-    #pragma unroll
-    for (int k = 0; k < (N * 9 + 31) / 32; ++k) {
-        const int i = lane + 32 * k, r = i / 9, j = i - 9 * r;
-        const uint8_t *row = b.src + (r0 + r) * b.stride;
-        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15u);
-        const uint8_t *at = row - off + 16 * j;
-        const bool want = i < N * 9 && r0 + r < b.rows && 16 * j < off + valid, whole = at >= b.lo && at + 16 <= b.hi;
-        if (want && whole) emmy::cp_async16(to + r * kStagedRow + 16 * j, at);
-        if (want && !whole) *reinterpret_cast<uint4 *>(staged + r * kStagedRow + 16 * j) = load_edge_word(at, b.lo, b.hi);
-    }
-}
-
 // The first `keep` bytes of a word (below 0 counts as 0).
 __device__ __forceinline__ uint32_t keep_bytes(uint32_t v, int keep) {
     return keep >= 4 ? v : keep <= 0 ? 0u : v & ((1u << (8 * keep)) - 1u);
 }
 
-// Cut the staged rows into the swizzled 128-byte rows of `operand`, zeros where nothing is wanted; one
-// warp, the one that staged them.
+// N rows from `r0` on into the swizzled 128-byte rows of `operand`, zeros where nothing is wanted; one
+// warp, 8 lanes to a row.  All loads are issued before the first is used, unless some word of the
+// warp lies across an end of the operand.
 template <int N>
-__device__ __forceinline__ void cut_rows(const Rows &b, int r0, const uint8_t *staged, uint8_t *operand, int lane) {
-    const int valid = static_cast<int>(b.valid < 128 ? b.valid : 128), j = lane & 7;
+__device__ __forceinline__ void copy_rows(const Rows &b, int r0, uint8_t *operand, int lane) {
+    constexpr int K = N / 4;
+    const int valid = static_cast<int>(b.valid < 128 ? b.valid : 128), j = lane & 7, have = valid - 16 * j;
+    const int rows = static_cast<int>(b.rows < r0 + N ? b.rows : r0 + N);
     const uint32_t low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(b.src)), low_stride = static_cast<uint32_t>(b.stride);
+    uint4 w0[K], w1[K];
+    bool edge = false;
+    const uint8_t *src = b.src + (r0 + (lane >> 3)) * b.stride + 16 * j;
     #pragma unroll
-    for (int k = 0; k < N / 4; ++k) {
-        const int r = (lane >> 3) + 4 * k, row = r0 + r, have = row < b.rows ? valid - 16 * j : 0;
+    for (int k = 0; k < K; ++k, src += 4 * b.stride) {
+        const int row = r0 + (lane >> 3) + 4 * k, off = static_cast<int>(low + row * low_stride) & 15;
+        const uint8_t *at = src - off;
+        const bool first = row < rows && have > 0, second = first && off + have > 16 && off > 0;
+        edge |= first && (at < b.lo || at + (second ? 32 : 16) > b.hi);
+    }
+    if (!__any_sync(0xffffffffu, edge)) {
+        src = b.src + (r0 + (lane >> 3)) * b.stride + 16 * j;
+        #pragma unroll
+        for (int k = 0; k < K; ++k, src += 4 * b.stride) {
+            const int row = r0 + (lane >> 3) + 4 * k, off = static_cast<int>(low + row * low_stride) & 15;
+            const uint4 *at = reinterpret_cast<const uint4 *>(src - off);
+            const bool first = row < rows && have > 0, second = first && off + have > 16 && off > 0;
+            w0[k] = first ? __ldg(at) : make_uint4(0, 0, 0, 0);
+            w1[k] = second ? __ldg(at + 1) : make_uint4(0, 0, 0, 0);
+        }
+    } else {
+        #pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int row = r0 + (lane >> 3) + 4 * k, off = static_cast<int>(low + row * low_stride) & 15;
+            const uint8_t *at = b.src + row * b.stride + 16 * j - off;
+            const bool first = row < rows && have > 0;
+            w0[k] = first ? load_edge_word(at, b.lo, b.hi) : make_uint4(0, 0, 0, 0);
+            w1[k] = first ? load_edge_word(at + 16, b.lo, b.hi) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    #pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int row = r0 + (lane >> 3) + 4 * k;
         const uint32_t off = low + row * low_stride;  // its low 4 bits count
-        const uint4 *w = reinterpret_cast<const uint4 *>(staged + r * kStagedRow + 16 * j);
-        const uint4 w0 = w[0], w1 = w[1];
-        const uint32_t a[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        const uint32_t a[8] = {w0[k].x, w0[k].y, w0[k].z, w0[k].w, w1[k].x, w1[k].y, w1[k].z, w1[k].w};
         uint32_t h[6], v[5], c[4];
         #pragma unroll
         for (int q = 0; q < 6; ++q) h[q] = off & 8u ? a[q + 2] : a[q];
         #pragma unroll
         for (int q = 0; q < 5; ++q) v[q] = off & 4u ? h[q + 1] : h[q];
         #pragma unroll
-        for (int q = 0; q < 4; ++q) c[q] = __funnelshift_r(v[q], v[q + 1], (off & 3u) * 8u);
-        if (have < 16) {
-            #pragma unroll
-            for (int q = 0; q < 4; ++q) c[q] = keep_bytes(c[q], have - 4 * q);
+        for (int q = 0; q < 4; ++q) {
+            c[q] = __funnelshift_r(v[q], v[q + 1], (off & 3u) * 8u);
+            if (have < 16) c[q] = keep_bytes(c[q], have - 4 * q);
         }
         *reinterpret_cast<uint4 *>(operand + row * kBlockBytes + ((j ^ (row & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
     }
@@ -493,18 +492,16 @@ struct TcConfig {
     static constexpr uint32_t kStageB = BN * kBlockBytes;
     static constexpr uint32_t kStage = kStageA + kStageB;
     static constexpr uint32_t kRed = BN * kTileM * 4;  // partial sums for the cluster
-    static constexpr int kStages = !TMA ? (BN == 32 ? 3 : 2) : BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
-    static constexpr int kStaged = !TMA ? (BN == 32 ? 4 : 2) : 0;  // blocks on their way to be cut into place
-    static constexpr uint32_t kStagedBytes = (kTileM + BN) * kStagedRow;
+    static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
     static constexpr int kOut = BN >= 64 && TMA ? 8 : 4;  // warps that turn sums into output
-    static constexpr int kLoaders = TMA ? 0 : 8;  // warps that load without TMA
+    static constexpr int kLoaders = TMA ? 0 : 16;  // warps that load without TMA, 8 to a block
     static constexpr int kThreads = 64 + 32 * (kOut + kLoaders);
-    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + kStaged * kStagedBytes + 256;
+    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + 256;
     static constexpr int kPerSm = TMA && BN <= 32 ? 2 : 1;  // CTAs that share an SM
     static constexpr uint32_t kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
-// Warp 0 loads operand tiles by TMA (TMA false: the last 8 warps load those operands whose rows
+// Warp 0 loads operand tiles by TMA (TMA false: the last 16 warps load those operands whose rows
 // TMA cannot take), warp 1 issues the MMAs into one of two accumulators, the warps from 2 on
 // turn the other into output, 4 or 8 of them: a warp reaches 32 of the 128 lanes.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
 // added in rank order: each CTA finishes its share of the columns, for which the others send their
@@ -524,8 +521,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
     uint8_t *sA = smem;
     uint8_t *sB = sA + STAGES * kStageA;
     uint32_t *red = reinterpret_cast<uint32_t *>(sB + STAGES * Cfg::kStageB);
-    uint8_t *staged = reinterpret_cast<uint8_t *>(red) + Cfg::kRed;
-    uint64_t *full = reinterpret_cast<uint64_t *>(staged + Cfg::kStaged * Cfg::kStagedBytes);
+    uint64_t *full = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(red) + Cfg::kRed);
     uint64_t *empty = full + STAGES;
     uint64_t *tfull = empty + STAGES;
     uint64_t *tempty = tfull + 2;
@@ -537,7 +533,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
 
     if (threadIdx.x == 64) {
         for (int s = 0; s < STAGES; ++s) {
-            emmy::mbar_init(&full[s], 1 + Cfg::kLoaders);
+            emmy::mbar_init(&full[s], 1 + Cfg::kLoaders / 2);
             emmy::mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -618,11 +614,12 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 ok = __all_sync(0xffffffffu, ok);
             }
         } else if (!TMA && warp >= 2 + Cfg::kOut) {
-            // Each of the 8 warps has 16 rows of A and BN / 8 of B to itself: it stages and cuts them
-            // without waiting for the others.  Rows run along m (c), or along k in panels of 64.
-            const int lw = warp - 2 - Cfg::kOut, slot0 = lw * 16, slotb0 = lw * (BN / 8);
+            // Two teams of 8 warps take every other block, so that one's loads are on their way while
+            // the other's are put in place.  A warp has 16 rows of A and BN / 8 of B; rows run along
+            // m (c), or along k in panels of 64.
+            const int lw = warp - 2 - Cfg::kOut, slot0 = (lw & 7) * 16, slotb0 = (lw & 7) * (BN / 8);
+            const uint32_t team = lw >> 3;
             const bool has_a = !flags.tma_a, has_b = !flags.tma_b;
-            constexpr int DEPTH = TMA ? 1 : Cfg::kStaged;
             constexpr int64_t ES = sizeof(T);
             for (int t = first; t < last && ok; t += step) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
@@ -659,38 +656,19 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                     }
                     return r;
                 };
-                auto staging = [&](int kb) { return staged + kb % DEPTH * Cfg::kStagedBytes; };
-                auto stage_block = [&](int kb) {
-                    if (kb < w.kb1) {
-                        if (has_a) stage_rows<16>(rows_a(kb), slot0, staging(kb) + slot0 * kStagedRow, lane);
-                        if (has_b)
-                            stage_rows<BN / 8>(rows_b(kb), slotb0, staging(kb) + (kTileM + slotb0) * kStagedRow, lane);
-                    }
-                    emmy::cp_async_commit();
-                };
-                for (int i = 0; i < DEPTH; ++i) stage_block(w.kb0 + i);
-                for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    emmy::cp_async_wait<DEPTH - 1>();
-                    ok = __all_sync(0xffffffffu, emmy::mbar_wait(&empty[stage], phase ^ 1u, abort_flag,
+                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+                    // `it` counts this CTA's blocks
+                    const uint32_t s = it % STAGES, sphase = it / STAGES & 1u;
+                    if ((it & 1u) != team) continue;
+                    ok = __all_sync(0xffffffffu, emmy::mbar_wait(&empty[s], sphase ^ 1u, abort_flag,
                                                                  EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs));
                     if (!ok) break;
-                    __syncwarp();  // what the other lanes loaded is here too
-                    if (has_a)
-                        cut_rows<16>(rows_a(kb), slot0, staging(kb) + slot0 * kStagedRow, sA + stage * kStageA, lane);
-                    if (has_b)
-                        cut_rows<BN / 8>(rows_b(kb), slotb0, staging(kb) + (kTileM + slotb0) * kStagedRow,
-                                 sB + stage * Cfg::kStageB, lane);
+                    if (has_a) copy_rows<16>(rows_a(kb), slot0, sA + s * kStageA, lane);
+                    if (has_b) copy_rows<(BN >= 32 ? BN / 8 : 4)>(rows_b(kb), slotb0, sB + s * Cfg::kStageB, lane);
                     emmy::fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) emmy::mbar_arrive(&full[stage]);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                    stage_block(kb + DEPTH);
+                    if (lane == 0) emmy::mbar_arrive(&full[s]);
                 }
-                emmy::cp_async_wait<0>();
-                __syncwarp();
             }
         } else if (warp == 1) {
             const Issue<I8, LAYOUT, false> issue(sA, sB, flags.bf16, BN);
