@@ -105,10 +105,37 @@ __device__ __forceinline__ void fence_proxy_async() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// 3-D tiled store from this CTA's shared memory, in the bulk group that the issuing thread commits next.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int32_t x, int32_t y, int32_t z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+// Ends a bulk group of this thread, which may be empty.
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The stores of all but this thread's N latest groups have read their shared memory.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // Programmatic launches: a kernel may start while the one before it on the stream still runs; it
 // waits here, before its first access to memory that others write, until that one has finished.
 __device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// 32 lanes x 16 consecutive 32-bit columns, back into tensor memory.
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
@@ -140,6 +167,7 @@ constexpr uint32_t kStageA = kTileM * kBlockBytes;
 struct Flags {
     bool bf16;            // 16-bit operands are bf16, else f16
     bool tma_a, tma_b;    // TMA can load the operand
+    bool tma_out;         // and store the output (16-bit outputs)
 };
 
 // The operands' layouts: which of them are contiguous along m (c) instead of along k.
@@ -373,9 +401,8 @@ __device__ __forceinline__ float scaled(uint32_t bits, float row_scale, const Ch
     else return sum_value<false>(bits);
 }
 
-// Staging of a warp's 32 channels x 32 output rows: 64 bytes a row, 80 apart, so that neither the
-// transposed 8 x 8 stores nor the 16-byte reads meet bank conflicts.
-constexpr uint32_t kStoreRow = 80, kStoreBytes = 32 * kStoreRow;
+// Staging of a warp's 32 channels x 16 output rows, twice.
+constexpr uint32_t kStoreRows = 16 * 64, kStoreBytes = 2 * kStoreRows;
 
 __device__ __forceinline__ uint32_t pack16(bool bf16, float lo, float hi) {
     if (bf16) {
@@ -388,13 +415,14 @@ __device__ __forceinline__ uint32_t pack16(bool bf16, float lo, float hi) {
 
 // Output rows [from, to) of a warp's 32 channels, from the accumulator at `taddr`.  Its channels lie
 // on lanes, the output's along a row.  16-bit outputs are transposed on the way: fragments of 8 x 8
-// go to shared memory through stmatrix, and 4 lanes then write each 64-byte piece of an output row
-// 16 bytes at a time (4 stores for 32 rows instead of 32, and the conversion packs two values).  f32
-// outputs need no help: 32 lanes write 128 bytes of a row.  `empty`: the sum had no terms.
+// go to shared memory through stmatrix, 16 rows of 64 bytes at a time, and from there to memory by
+// TMA, which leaves the warp free to turn to the next 16.  Rows that TMA may not write whole (the
+// group ends among them) or cannot address are written by the warp.  f32 outputs need no help: 32
+// lanes write 128 bytes of a row.  `empty`: the sum had no terms.
 template <bool I8, int N>
-__device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int mq, uint32_t taddr, bool empty, int from,
-                                           const Channel &own, RowScales<I8, N> xs, uint8_t *buf, int lane) {
-    const int to = min(from + 32 * N, w.cols);
+__device__ __forceinline__ void store_tile(const Product &p, const CUtensorMap *out_map, const Tile &w, int mq,
+                                           uint32_t taddr, bool empty, int from, int to, const Channel &own,
+                                           RowScales<I8, N> xs, uint8_t *buf, int lane) {
     if (p.out_type == EMMY_F32) {
         const int64_t m = mq + lane;
         float *out = static_cast<float *>(p.out) + out_index(p, w, m, from);
@@ -417,9 +445,7 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
         return;
     }
     const int piece = lane & 3;
-    uint16_t *out = static_cast<uint16_t *>(p.out) + out_index(p, w, mq, from);
-    const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && ((p.out_c | p.out_e | p.m) & 7) == 0;
-    const bool bf16 = p.out_type == EMMY_BF16, piece_in = mq + piece * 8 < p.m;
+    const bool bf16 = p.out_type == EMMY_BF16;
     Channel ch[4];
     if constexpr (I8) {
         #pragma unroll
@@ -428,9 +454,10 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
             ch[i].bias = __shfl_sync(0xffffffffu, own.bias, lane / 4 + 8 * i);
         }
     }
+    const int in_row = (lane >> 4) * 8 + (lane & 7), y0 = p.dw ? w.c0 : w.begin + w.c0, z = p.dw ? w.e : 0;
     #pragma unroll 1
-    for (int c = from; c < to; c += 32, out += 32 * p.out_c, xs.next()) {
-        uint32_t r[2][16];
+    for (int c = from; c < to; c += 32, xs.next()) {
+        uint32_t r[2][16], v[2][8];
         emmy::tmem_ld_16x256b_x4(taddr + c, r[0]);
         emmy::tmem_ld_16x256b_x4(taddr + (16u << 16) + c, r[1]);
         float x[8];
@@ -443,31 +470,41 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
         }
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t v[8];
             #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int row = 2 * h + (i & 1), col = i >> 1 << 1;
-                v[i] = pack16(bf16, scaled<I8>(r[h][2 * i], x[col], ch[row]), scaled<I8>(r[h][2 * i + 1], x[col + 1], ch[row]));
+                v[h][i] = pack16(bf16, scaled<I8>(r[h][2 * i], x[col], ch[row]), scaled<I8>(r[h][2 * i + 1], x[col + 1], ch[row]));
             }
-            const uint32_t at = emmy::smem_u32(buf) + ((lane >> 4) * 8 + (lane & 7)) * kStoreRow +
-                                (16 * h + 8 * ((lane >> 3) & 1)) * 2;
-            emmy::stmatrix_x4_trans(at, v[0], v[1], v[2], v[3]);
-            emmy::stmatrix_x4_trans(at + 16 * kStoreRow, v[4], v[5], v[6], v[7]);
         }
-        __syncwarp();
-        if (vec) {
+        #pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            // 16 rows, with the 16-byte chunks of each exchanged as TMA's 64-byte swizzle does
+            uint8_t *rows16 = buf + half * kStoreRows;
+            const int c16 = c + 16 * half;
+            if (c16 >= to) break;
+            if (lane == 0) emmy::tma_store_wait_read<1>();  // the store before last has left this half
+            __syncwarp();
             #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = i * 8 + (lane >> 2);
-                if (piece_in && c + row < to)
-                    *reinterpret_cast<uint4 *>(out + row * p.out_c + piece * 8) =
-                        *reinterpret_cast<const uint4 *>(buf + row * kStoreRow + piece * 16);
+            for (int h = 0; h < 2; ++h) {
+                const int chunk = (2 * h + ((lane >> 3) & 1)) ^ ((in_row >> 1) & 3);
+                emmy::stmatrix_x4_trans(emmy::smem_u32(rows16) + in_row * 64 + chunk * 16, v[h][4 * half], v[h][4 * half + 1],
+                                        v[h][4 * half + 2], v[h][4 * half + 3]);
             }
-        } else if (mq + lane < p.m) {
-            for (int row = 0; row < 32 && c + row < to; ++row)
-                out[row * p.out_c + lane] = *reinterpret_cast<const uint16_t *>(buf + row * kStoreRow + lane * 2);
+            if (out_map && (p.dw || c16 + 16 <= to)) {
+                emmy::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0 && mq < p.m) emmy::tma_store_3d(out_map, emmy::smem_u32(rows16), mq, y0 + c16, z);
+            } else {
+                __syncwarp();
+                uint16_t *out = static_cast<uint16_t *>(p.out) + out_index(p, w, mq + lane, c16);
+                if (mq + lane < p.m)
+                    for (int i = 0; i < 16 && c16 + i < to; ++i, out += p.out_c)
+                        *out = *reinterpret_cast<const uint16_t *>(rows16 + i * 64 + ((lane >> 3) ^ ((i >> 1) & 3)) * 16 +
+                                                                   (lane & 7) * 2);
+                __syncwarp();
+            }
+            if (lane == 0) emmy::tma_store_commit();  // one group for each half, stored or not
         }
-        __syncwarp();
     }
 }
 
@@ -492,13 +529,15 @@ struct TcConfig {
     static constexpr uint32_t kStageB = BN * kBlockBytes;
     static constexpr uint32_t kStage = kStageA + kStageB;
     static constexpr uint32_t kRed = BN * kTileM * 4;  // partial sums for the cluster
-    static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 7 : 4;
+    static constexpr uint32_t kOutStage = BN >= 64 ? 4 * kStoreBytes * (TMA ? 2 : 1) : 0;
+    static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 6 : 4;
     static constexpr int kOut = BN >= 64 && TMA ? 8 : 4;  // warps that turn sums into output
     static constexpr int kLoaders = TMA ? 0 : 16;  // warps that load without TMA, 8 to a block
     static constexpr int kThreads = 64 + 32 * (kOut + kLoaders);
-    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + 256;
+    static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + kOutStage + 256;
     static constexpr int kPerSm = TMA && BN <= 32 ? 2 : 1;  // CTAs that share an SM
-    static constexpr uint32_t kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
+    // two accumulators; store_tile reads 32 columns at a time, which may pass the second one's end
+    static constexpr uint32_t kTmemCols = BN >= 64 ? 4 * BN : 2 * BN;
 };
 
 // Warp 0 loads operand tiles by TMA (TMA false: the last 16 warps load those operands whose rows
@@ -509,7 +548,7 @@ struct TcConfig {
 template <bool I8, int LAYOUT, int BN, bool TMA>
 __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, BN, TMA>::kPerSm)
     product_tc_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
-                      const __grid_constant__ CUtensorMap tm_b) {
+                      const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out) {
     using Cfg = TcConfig<I8, BN, TMA>;
     using T = std::conditional_t<I8, int8_t, uint16_t>;
     static_assert(LAYOUT != kMM || BN % 64 == 0, "dw's B comes in panels of 64");
@@ -521,7 +560,8 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
     uint8_t *sA = smem;
     uint8_t *sB = sA + STAGES * kStageA;
     uint32_t *red = reinterpret_cast<uint32_t *>(sB + STAGES * Cfg::kStageB);
-    uint64_t *full = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(red) + Cfg::kRed);
+    uint8_t *out_stage = reinterpret_cast<uint8_t *>(red) + Cfg::kRed;
+    uint64_t *full = reinterpret_cast<uint64_t *>(out_stage + Cfg::kOutStage);
     uint64_t *empty = full + STAGES;
     uint64_t *tfull = empty + STAGES;
     uint64_t *tempty = tfull + 2;
@@ -569,6 +609,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
     uint32_t stage = 0, phase = 0, it = 0;
     uint32_t issued = 0u, parity_bits = 0u;  // producer: loads in flight for each stage and their parity
     bool ok = true;
+    const CUtensorMap *out_map = flags.tma_out ? &tm_out : nullptr;
     const uint32_t share = BN / split, share_log = 31 - __clz(share);  // columns of a tile that each CTA finishes
     int e = 0;
     // Without a cluster each role runs through all of the CTA's tiles at its own pace; a cluster
@@ -726,9 +767,8 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
                 const bool none = w.kb0 == w.kb1;  // nothing was accumulated
                 if (BN >= 64 && split == 1) {
-                    // the sums' exchange buffer is free without a cluster
-                    store_tile<I8>(p, w, w.m0 + q * 32, taddr, none, part * SPAN, ch, xs,
-                                   reinterpret_cast<uint8_t *>(red) + (warp - 2) * kStoreBytes, lane);
+                    store_tile<I8>(p, out_map, w, w.m0 + q * 32, taddr, none, part * SPAN, min((part + 1) * SPAN, w.cols), ch, xs,
+                                   out_stage + (warp - 2) * kStoreBytes, lane);
                 } else {
                     // few columns, or parts of sums: channels of a column are neighbours either way
                     if (!met) {
@@ -780,11 +820,40 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 met = true;
             }
             emmy::cluster_sync();  // this CTA's columns have arrived from every rank
-            if (out_warp) {
+            if (out_warp && BN >= 64) {
+                // sums go back to tensor memory, where a whole tile's would be, and leave the same way
+                const uint32_t acc = (it - 1) & 1u;
+                const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + acc * BN;
+                const int span = max(static_cast<int>(share) / parts, 32), begin = from + part * span;
+                const int to = min(min(begin + span, from + static_cast<int>(share)), w.cols);
+                #pragma unroll 1
+                for (int c = begin; c < to; c += 16) {
+                    uint32_t sum[16];
+                    const uint32_t *at = red + (c - from) * kTileM + lm;
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[j] = at[j * kTileM];
+                    for (uint32_t s = 1; s < split; ++s) {
+                        at += share * kTileM;
+                        #pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const uint32_t v = at[j * kTileM];
+                            sum[j] = I8 ? sum[j] + v : __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(v));
+                        }
+                    }
+                    emmy::tmem_st_32x32b_x16(taddr + c, sum);
+                }
+                emmy::tmem_st_wait();
+                __syncwarp();
+                if (begin < to) {
+                    const RowScales<I8, 2> scales(p, w, begin, lane);
+                    store_tile<I8>(p, out_map, w, w.m0 + (warp & 3) * 32, taddr, false, begin, to, ch, scales,
+                                   out_stage + (warp - 2) * kStoreBytes, lane);
+                }
+            } else if (out_warp) {
                 const int64_t m = w.m0 + lm;
                 const int to = min(from + static_cast<int>(share), w.cols);
                 #pragma unroll 4
-                for (int c = from + part; c < to; c += parts) {
+                for (int c = from; c < to; ++c) {
                     const uint32_t *at = red + (c - from) * kTileM + lm;
                     uint32_t v[8], sum = 0u;  // 0 of either type
                     #pragma unroll
@@ -793,8 +862,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                     for (int s = 0; s < 8; ++s)
                         if (s < split)
                             sum = I8 ? sum + v[s] : __float_as_uint(__uint_as_float(sum) + __uint_as_float(v[s]));
-                    float x = 0.0f;
-                    if constexpr (I8) x = c - from < 32 ? __shfl_sync(0xffffffffu, xs, c - from) : p.x_scale[w.begin + w.c0 + c];
+                    const float x = I8 ? __shfl_sync(0xffffffffu, xs, c - from) : 0.0f;
                     if (m < p.m) store_out(p.out, p.out_type, out_index(p, w, m, c), scaled<I8>(sum, x, ch));
                 }
             }
@@ -803,6 +871,10 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 emmy::cluster_sync();  // and may be overwritten
             }
         }
+    }
+    if (BN >= 64 && warp >= 2 && warp < 2 + Cfg::kOut) {
+        if (lane == 0) emmy::tma_store_wait();  // before the shared memory they read from goes
+        __syncwarp();
     }
     if (!met) {
         __syncwarp();
@@ -852,7 +924,7 @@ struct PairConfig {
 template <bool I8, int LAYOUT, int BN>
 __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
     product_pair_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
-                        const __grid_constant__ CUtensorMap tm_b) {
+                        const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out) {
     using Cfg = PairConfig<BN>;
     constexpr int STAGES = Cfg::kStages, BK = I8 ? 128 : 64, CN = BN / 2;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -1054,6 +1126,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
         const int q = warp & 3, part = (warp - 2) >> 2;
         constexpr int SPAN = BN / (Cfg::kOut / 4);
         const uint32_t leader_tempty = emmy::mapa(&tempty[0], 0);
+        const CUtensorMap *out_map = flags.tma_out ? &tm_out : nullptr;
         uint32_t it = 0;
         for (int t = pair; t < total; t += npairs, ++it) {
             const Tile w = tile(t);
@@ -1064,12 +1137,14 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
                                                                  EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)))
                 break;
             emmy::tc_fence_after();
-            store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
-                           part * SPAN, ch, xs, sStore + (warp - 2) * kStoreBytes, lane);
+            store_tile<I8>(p, out_map, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
+                           part * SPAN, min((part + 1) * SPAN, w.cols), ch, xs, sStore + (warp - 2) * kStoreBytes, lane);
             emmy::tc_fence_before();
             __syncwarp();
             if (lane == 0) emmy::mbar_arrive_cluster(leader_tempty + acc * 8u);
         }
+        if (lane == 0) emmy::tma_store_wait();  // before the shared memory they read from goes
+        __syncwarp();
     }
     emmy::tc_fence_before();
     __syncthreads();
