@@ -259,14 +259,14 @@ bool tma_ready(Operand &o, int esize) {
 }
 
 bool encode(CUtensorMap *map, const Operand &o, CUtensorMapDataType type, int esize, int rank, uint32_t box_inner,
-            uint32_t box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+            uint32_t box_rows) {
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.inner), static_cast<cuuint64_t>(o.rows),
                                 static_cast<cuuint64_t>(o.mats)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.row_stride) * esize,
                                    static_cast<cuuint64_t>(o.mat_stride) * esize};
     const cuuint32_t box[3] = {box_inner, box_rows, 1}, step[3] = {1, 1, 1};
     return encode_tiled()(map, type, rank, const_cast<void *>(o.base), dims, strides, box, step,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -304,14 +304,14 @@ cudaLaunchAttribute early_start() {
     return attr;
 }
 
-using TcKernel = void (*)(Product, Flags, CUtensorMap, CUtensorMap, CUtensorMap);
+using TcKernel = void (*)(Product, Flags, CUtensorMap, CUtensorMap);
 
 // What every variant's launch takes.
 struct Launch {
     const Call &call;
     const Product &p;
     Flags flags;
-    const CUtensorMap &ta, &tb, &tout;
+    const CUtensorMap &ta, &tb;
     int64_t clusters;
     int cluster;
 };
@@ -330,7 +330,7 @@ int launch_clusters(const Launch &l, TcKernel kernel, std::atomic<uint64_t> &rea
     attrs[1].val.clusterDim = {static_cast<unsigned>(l.cluster), 1, 1};
     cfg.attrs = attrs;
     cfg.numAttrs = 2;
-    return launched(l.call, cudaLaunchKernelEx(&cfg, kernel, l.p, l.flags, l.ta, l.tb, l.tout));
+    return launched(l.call, cudaLaunchKernelEx(&cfg, kernel, l.p, l.flags, l.ta, l.tb));
 }
 
 template <bool I8, int LAYOUT, int BN, bool TMA>
@@ -344,7 +344,8 @@ template <bool I8, int LAYOUT, int BN>
 int launch_pair(const Launch &l) {
     using Cfg = PairConfig<BN>;
     static std::atomic<uint64_t> ready{0};
-    return launch_clusters(l, product_pair_kernel<I8, LAYOUT, BN>, ready, Cfg::kThreads, Cfg::kSmem);
+    return launch_clusters(l, product_pair_kernel<I8, LAYOUT, BN>, ready,
+                           Cfg::kThreads + (LAYOUT == kMM ? Cfg::kTailThreads : 0), Cfg::kSmem);
 }
 
 template <bool I8, int LAYOUT>
@@ -387,10 +388,7 @@ int launch_product(const Call &call, Product p, bool bf16) {
     }
     p.a_end = end_of(a, esize);
     p.b_end = end_of(b, esize);
-    // TMA writes whole 16-byte pieces of a row, so a row that ends inside one is not its to write
-    Operand out{p.out, p.m, p.dw ? p.c : p.rows, p.out_c, p.dw ? p.experts : 1, p.out_e};
-    const Flags flags{bf16, encode_tiled() && tma_ready(a, esize), encode_tiled() && tma_ready(b, esize),
-                      encode_tiled() && p.out_type != EMMY_F32 && p.m % 8 == 0 && tma_ready(out, 2)};
+    const Flags flags{bf16, encode_tiled() && tma_ready(a, esize), encode_tiled() && tma_ready(b, esize)};
     const bool tma = flags.tma_a && flags.tma_b;
 
     // groups that can hold rows, and the rows of an even one
@@ -404,8 +402,11 @@ int launch_product(const Call &call, Product p, bool bf16) {
         return ceil_div(p.m, tm) * (p.dw ? p.experts * ceil_div(p.c, tc) : p.rows / tc + groups);
     };
     const int64_t cext = p.dw ? p.c : even;
+    // Pairs of CTAs where groups have rows for them and there are tiles enough, and, for dw, where the
+    // sums are long enough to cover a wide tile's way out (32 experts, dw [512, 1024]: 256 rows each 22
+    // against a single CTA's 19 us, 1000 rows each of 16 [1024, 1024] 36 against 47 us).
     int pair = 0;
-    if (tma && p.m > 128 && cext > 64) {
+    if (tma && p.m > 128 && cext > 64 && !(p.dw && kblocks < 8)) {
         if (cext > 128 && tiles(256, 256) >= kSms / 4) pair = 256;
         else if (tiles(256, 128) >= kSms / 4) pair = 128;
     }
@@ -413,23 +414,30 @@ int launch_product(const Call &call, Product p, bool bf16) {
         return report(EMMY_ERR_INVALID, "%s: an output of more than 2^31 tiles is not supported", call.name);
     const int bn = pair ? pair : p.dw ? 128 : !tma ? (even <= 24 ? 32 : 128) : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
 
-    CUtensorMap ta{}, tb{}, tout{};
+    CUtensorMap ta{}, tb{};
     const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                      : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if ((flags.tma_a && !encode(&ta, a, type, esize, 3, bk, a_mn ? 64 : kTileM)) ||
-        (flags.tma_b && !encode(&tb, b, type, esize, 2, bk, p.dw ? 64 : pair ? pair / 2 : bn)) ||
-        (flags.tma_out && !encode(&tout, out, p.out_type == EMMY_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                                  2, 3, 32, 16, CU_TENSOR_MAP_SWIZZLE_64B)))
+        (flags.tma_b && !encode(&tb, b, type, esize, 2, bk, p.dw ? 64 : pair ? pair / 2 : bn)))
         return report(EMMY_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", call.name);
-    const int resident = pair ? kSms : kSms * (tma && bn <= 32 ? 2 : 1);
+    // CTAs that run at once: clusters of 4 and 8 leave some of a GPC's SMs over
+    auto resident = [&](int cluster) {
+        const int per_sm = !pair && tma && bn <= 32 ? 2 : 1;
+        return per_sm * (cluster <= 2 ? kSms : cluster == 4 ? 132 : 120);
+    };
+    // Idle SMs take parts of the sums, as long as a part is worth the exchange: 4 blocks of it for
+    // the few columns of a narrow tile, 16 for a wide one (1022 rows, 8 experts, dx [1000, 776], 13
+    // blocks: 11 us whole, 18 in halves; 60000 rows, dw [256, 256]: 275 us whole, 42 in eighths).
     int split = 1;
     if (!pair)
-        while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident && kblocks >= split * 2 * 4) split *= 2;
+        while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident(split * 2) &&
+               kblocks >= split * 2 * (bn <= 32 ? 4 : 16))
+            split *= 2;
     const int cluster = pair ? 2 : split;
     int64_t clusters = pair ? most(2 * kTileM, pair) : most(kTileM, bn);
-    if (clusters > resident / cluster) clusters = resident / cluster;
-    const Launch l{call, p, flags, ta, tb, tout, clusters, cluster};
+    if (clusters > resident(cluster) / cluster) clusters = resident(cluster) / cluster;
+    const Launch l{call, p, flags, ta, tb, clusters, cluster};
     if constexpr (I8) {
         return launch_variant<true, kKK>(l, tma, pair, bn);
     } else {

@@ -105,22 +105,6 @@ __device__ __forceinline__ void fence_proxy_async() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// 3-D tiled store from this CTA's shared memory, in the bulk group that the issuing thread commits next.
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int32_t x, int32_t y, int32_t z) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
-                     reinterpret_cast<uint64_t>(map)),
-                 "r"(src), "r"(x), "r"(y), "r"(z)
-                 : "memory");
-}
-// Ends a bulk group of this thread, which may be empty.
-__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// The stores of all but this thread's N latest groups have read their shared memory.
-template <int N>
-__device__ __forceinline__ void tma_store_wait_read() {
-    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
 // Programmatic launches: a kernel may start while the one before it on the stream still runs; it
 // waits here, before its first access to memory that others write, until that one has finished.
 __device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -167,7 +151,6 @@ constexpr uint32_t kStageA = kTileM * kBlockBytes;
 struct Flags {
     bool bf16;            // 16-bit operands are bf16, else f16
     bool tma_a, tma_b;    // TMA can load the operand
-    bool tma_out;         // and store the output (16-bit outputs)
 };
 
 // The operands' layouts: which of them are contiguous along m (c) instead of along k.
@@ -401,8 +384,9 @@ __device__ __forceinline__ float scaled(uint32_t bits, float row_scale, const Ch
     else return sum_value<false>(bits);
 }
 
-// Staging of a warp's 32 channels x 16 output rows, twice.
-constexpr uint32_t kStoreRows = 16 * 64, kStoreBytes = 2 * kStoreRows;
+// Staging of a warp's 32 channels x 32 output rows: 64 bytes a row, 80 apart, so that neither the
+// transposed 8 x 8 stores nor the 16-byte reads meet bank conflicts.
+constexpr uint32_t kStoreRow = 80, kStoreBytes = 32 * kStoreRow;
 
 __device__ __forceinline__ uint32_t pack16(bool bf16, float lo, float hi) {
     if (bf16) {
@@ -415,37 +399,41 @@ __device__ __forceinline__ uint32_t pack16(bool bf16, float lo, float hi) {
 
 // Output rows [from, to) of a warp's 32 channels, from the accumulator at `taddr`.  Its channels lie
 // on lanes, the output's along a row.  16-bit outputs are transposed on the way: fragments of 8 x 8
-// go to shared memory through stmatrix, 16 rows of 64 bytes at a time, and from there to memory by
-// TMA, which leaves the warp free to turn to the next 16.  Rows that TMA may not write whole (the
-// group ends among them) or cannot address are written by the warp.  f32 outputs need no help: 32
-// lanes write 128 bytes of a row.  `empty`: the sum had no terms.
+// go to shared memory through stmatrix, and 4 lanes then write each 64-byte piece of an output row
+// 16 bytes at a time (4 stores for 32 rows instead of 32, and the conversion packs two values).
+// f32 outputs need no help: 32 lanes write 128 bytes of a row.  The next columns come from tensor
+// memory while these are stored.  A 32 x 32 piece takes a warp about 800 cycles (300 to convert, 180
+// through stmatrix, 330 for the reads and stores); TMA stores of two 32 x 16 pieces took 1250, most of
+// it in issuing them from one lane.
+// `empty`: the sum had no terms.
 template <bool I8, int N>
-__device__ __forceinline__ void store_tile(const Product &p, const CUtensorMap *out_map, const Tile &w, int mq,
-                                           uint32_t taddr, bool empty, int from, int to, const Channel &own,
-                                           RowScales<I8, N> xs, uint8_t *buf, int lane) {
+__device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int mq, uint32_t taddr, bool empty, int from,
+                                           int to, const Channel &own, RowScales<I8, N> xs, uint8_t *buf, int lane) {
     if (p.out_type == EMMY_F32) {
         const int64_t m = mq + lane;
         float *out = static_cast<float *>(p.out) + out_index(p, w, m, from);
+        uint32_t r[32];
+        if (from < to) emmy::tmem_ld_32x32b_x32(taddr + from, r);
         #pragma unroll 1
         for (int c = from; c < to; c += 32, out += 32 * p.out_c, xs.next()) {
-            uint32_t r[32];
-            emmy::tmem_ld_32x32b_x32(taddr + c, r);
+            float v[32];
             emmy::tmem_ld_wait();
-            if (empty) {
-                #pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = 0u;
-            }
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = scaled<I8>(empty ? 0u : r[j], xs.at(j), own);
+            if (c + 32 < to) emmy::tmem_ld_32x32b_x32(taddr + c + 32, r);  // on their way while these are stored
             float *o = out;
             #pragma unroll
-            for (int j = 0; j < 32; ++j, o += p.out_c) {
-                const float v = scaled<I8>(r[j], xs.at(j), own);
-                if (m < p.m && c + j < to) *o = v;
-            }
+            for (int j = 0; j < 32; ++j, o += p.out_c)
+                if (m < p.m && c + j < to) *o = v[j];
         }
         return;
     }
-    const int piece = lane & 3;
-    const bool bf16 = p.out_type == EMMY_BF16;
+    const int piece = lane & 3, row4 = lane >> 2;
+    const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && ((p.out_c | p.out_e | p.m) & 7) == 0;
+    const bool bf16 = p.out_type == EMMY_BF16, in = vec ? mq + piece * 8 < p.m : mq + lane < p.m;
+    const int64_t step8 = 8 * p.out_c;
+    uint16_t *out = static_cast<uint16_t *>(p.out) +
+                    (vec ? out_index(p, w, mq + piece * 8, from + row4) : out_index(p, w, mq + lane, from));
     Channel ch[4];
     if constexpr (I8) {
         #pragma unroll
@@ -454,12 +442,16 @@ __device__ __forceinline__ void store_tile(const Product &p, const CUtensorMap *
             ch[i].bias = __shfl_sync(0xffffffffu, own.bias, lane / 4 + 8 * i);
         }
     }
-    const int in_row = (lane >> 4) * 8 + (lane & 7), y0 = p.dw ? w.c0 : w.begin + w.c0, z = p.dw ? w.e : 0;
+    const uint32_t put = emmy::smem_u32(buf) + ((lane >> 4) * 8 + (lane & 7)) * kStoreRow + 16 * ((lane >> 3) & 1);
+    const uint8_t *get = buf + row4 * kStoreRow + piece * 16;
+    uint32_t r[2][16];
+    if (from < to) {
+        emmy::tmem_ld_16x256b_x4(taddr + from, r[0]);
+        emmy::tmem_ld_16x256b_x4(taddr + (16u << 16) + from, r[1]);
+    }
     #pragma unroll 1
     for (int c = from; c < to; c += 32, xs.next()) {
-        uint32_t r[2][16], v[2][8];
-        emmy::tmem_ld_16x256b_x4(taddr + c, r[0]);
-        emmy::tmem_ld_16x256b_x4(taddr + (16u << 16) + c, r[1]);
+        uint32_t v[2][8];
         float x[8];
         #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = xs.at(8 * (i >> 1) + 2 * piece + (i & 1));
@@ -476,35 +468,28 @@ __device__ __forceinline__ void store_tile(const Product &p, const CUtensorMap *
                 v[h][i] = pack16(bf16, scaled<I8>(r[h][2 * i], x[col], ch[row]), scaled<I8>(r[h][2 * i + 1], x[col + 1], ch[row]));
             }
         }
-        #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            // 16 rows, with the 16-byte chunks of each exchanged as TMA's 64-byte swizzle does
-            uint8_t *rows16 = buf + half * kStoreRows;
-            const int c16 = c + 16 * half;
-            if (c16 >= to) break;
-            if (lane == 0) emmy::tma_store_wait_read<1>();  // the store before last has left this half
-            __syncwarp();
-            #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int chunk = (2 * h + ((lane >> 3) & 1)) ^ ((in_row >> 1) & 3);
-                emmy::stmatrix_x4_trans(emmy::smem_u32(rows16) + in_row * 64 + chunk * 16, v[h][4 * half], v[h][4 * half + 1],
-                                        v[h][4 * half + 2], v[h][4 * half + 3]);
-            }
-            if (out_map && (p.dw || c16 + 16 <= to)) {
-                emmy::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0 && mq < p.m) emmy::tma_store_3d(out_map, emmy::smem_u32(rows16), mq, y0 + c16, z);
-            } else {
-                __syncwarp();
-                uint16_t *out = static_cast<uint16_t *>(p.out) + out_index(p, w, mq + lane, c16);
-                if (mq + lane < p.m)
-                    for (int i = 0; i < 16 && c16 + i < to; ++i, out += p.out_c)
-                        *out = *reinterpret_cast<const uint16_t *>(rows16 + i * 64 + ((lane >> 3) ^ ((i >> 1) & 3)) * 16 +
-                                                                   (lane & 7) * 2);
-                __syncwarp();
-            }
-            if (lane == 0) emmy::tma_store_commit();  // one group for each half, stored or not
+        if (c + 32 < to) {  // on their way while these are stored
+            emmy::tmem_ld_16x256b_x4(taddr + c + 32, r[0]);
+            emmy::tmem_ld_16x256b_x4(taddr + (16u << 16) + c + 32, r[1]);
         }
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            emmy::stmatrix_x4_trans(put + 32 * h, v[h][0], v[h][1], v[h][2], v[h][3]);
+            emmy::stmatrix_x4_trans(put + 32 * h + 16 * kStoreRow, v[h][4], v[h][5], v[h][6], v[h][7]);
+        }
+        __syncwarp();
+        if (vec) {
+            uint4 q[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const uint4 *>(get + i * 8 * kStoreRow);
+            #pragma unroll
+            for (int i = 0; i < 4; ++i, out += step8)
+                if (in && c + i * 8 + row4 < to) *reinterpret_cast<uint4 *>(out) = q[i];
+        } else {
+            for (int i = 0; i < 32; ++i, out += p.out_c)
+                if (in && c + i < to) *out = *reinterpret_cast<const uint16_t *>(buf + i * kStoreRow + lane * 2);
+        }
+        __syncwarp();
     }
 }
 
@@ -532,7 +517,11 @@ struct TcConfig {
     static constexpr uint32_t kOutStage = BN >= 64 ? 4 * kStoreBytes * (TMA ? 2 : 1) : 0;
     static constexpr int kStages = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 6 : 4;
     static constexpr int kOut = BN >= 64 && TMA ? 8 : 4;  // warps that turn sums into output
-    static constexpr int kLoaders = TMA ? 0 : 16;  // warps that load without TMA, 8 to a block
+    // two teams on alternate blocks hide more of the loads' latency (8 rows of 8 experts, int8 [3425,
+    // 4057]: 94 against 125 us); with both operands 128 rows high they lack the registers (dw
+    // [777, 1001] of 1022 rows: 54 against 38 us)
+    static constexpr int kTeams = BN == 32 ? 2 : 1;
+    static constexpr int kLoaders = TMA ? 0 : 8 * kTeams;  // warps that load without TMA, 8 to a block
     static constexpr int kThreads = 64 + 32 * (kOut + kLoaders);
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + kOutStage + 256;
     static constexpr int kPerSm = TMA && BN <= 32 ? 2 : 1;  // CTAs that share an SM
@@ -548,7 +537,7 @@ struct TcConfig {
 template <bool I8, int LAYOUT, int BN, bool TMA>
 __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, BN, TMA>::kPerSm)
     product_tc_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
-                      const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out) {
+                      const __grid_constant__ CUtensorMap tm_b) {
     using Cfg = TcConfig<I8, BN, TMA>;
     using T = std::conditional_t<I8, int8_t, uint16_t>;
     static_assert(LAYOUT != kMM || BN % 64 == 0, "dw's B comes in panels of 64");
@@ -573,7 +562,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
 
     if (threadIdx.x == 64) {
         for (int s = 0; s < STAGES; ++s) {
-            emmy::mbar_init(&full[s], 1 + Cfg::kLoaders / 2);
+            emmy::mbar_init(&full[s], 1 + Cfg::kLoaders / Cfg::kTeams);
             emmy::mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -609,7 +598,6 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
     uint32_t stage = 0, phase = 0, it = 0;
     uint32_t issued = 0u, parity_bits = 0u;  // producer: loads in flight for each stage and their parity
     bool ok = true;
-    const CUtensorMap *out_map = flags.tma_out ? &tm_out : nullptr;
     const uint32_t share = BN / split, share_log = 31 - __clz(share);  // columns of a tile that each CTA finishes
     int e = 0;
     // Without a cluster each role runs through all of the CTA's tiles at its own pace; a cluster
@@ -700,7 +688,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
                     // `it` counts this CTA's blocks
                     const uint32_t s = it % STAGES, sphase = it / STAGES & 1u;
-                    if ((it & 1u) != team) continue;
+                    if (it % Cfg::kTeams != team) continue;
                     ok = __all_sync(0xffffffffu, emmy::mbar_wait(&empty[s], sphase ^ 1u, abort_flag,
                                                                  EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs));
                     if (!ok) break;
@@ -767,7 +755,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
                 const bool none = w.kb0 == w.kb1;  // nothing was accumulated
                 if (BN >= 64 && split == 1) {
-                    store_tile<I8>(p, out_map, w, w.m0 + q * 32, taddr, none, part * SPAN, min((part + 1) * SPAN, w.cols), ch, xs,
+                    store_tile<I8>(p, w, w.m0 + q * 32, taddr, none, part * SPAN, min((part + 1) * SPAN, w.cols), ch, xs,
                                    out_stage + (warp - 2) * kStoreBytes, lane);
                 } else {
                     // few columns, or parts of sums: channels of a column are neighbours either way
@@ -846,7 +834,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 __syncwarp();
                 if (begin < to) {
                     const RowScales<I8, 2> scales(p, w, begin, lane);
-                    store_tile<I8>(p, out_map, w, w.m0 + (warp & 3) * 32, taddr, false, begin, to, ch, scales,
+                    store_tile<I8>(p, w, w.m0 + (warp & 3) * 32, taddr, false, begin, to, ch, scales,
                                    out_stage + (warp - 2) * kStoreBytes, lane);
                 }
             } else if (out_warp) {
@@ -871,10 +859,6 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 emmy::cluster_sync();  // and may be overwritten
             }
         }
-    }
-    if (BN >= 64 && warp >= 2 && warp < 2 + Cfg::kOut) {
-        if (lane == 0) emmy::tma_store_wait();  // before the shared memory they read from goes
-        __syncwarp();
     }
     if (!met) {
         __syncwarp();
@@ -918,13 +902,14 @@ struct PairConfig {
     static constexpr int kStages = BN == 256 ? 6 : 8;
     static constexpr int kOut = 8;  // warps that turn sums into output
     static constexpr int kThreads = 64 + 32 * kOut;
+    static constexpr int kTailThreads = 32;  // dw: one more warp
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kOut * kStoreBytes + 512;
 };
 
 template <bool I8, int LAYOUT, int BN>
-__global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
+__global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? PairConfig<BN>::kTailThreads : 0), 1)
     product_pair_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
-                        const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out) {
+                        const __grid_constant__ CUtensorMap tm_b) {
     using Cfg = PairConfig<BN>;
     constexpr int STAGES = Cfg::kStages, BK = I8 ? 128 : 64, CN = BN / 2;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -938,27 +923,23 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
     uint64_t *tfull = empty + STAGES;
     uint64_t *tempty = tfull + 2;
     uint64_t *drain = tempty + 2;
-    uint64_t *tail = drain + 1;       // this CTA's loads of a block that ends inside
-    // the peer's are in and their spare rows zeroed (leader only); one for each stage, because the
-    // peer may be several blocks ahead, but never twice on one stage
-    uint64_t *tail_peer = tail + 1;
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(tail_peer + STAGES);
+    uint64_t *tail = drain + 1;  // for each stage: this CTA's loads of a block that ends inside
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(tail + STAGES);
     volatile uint32_t *abort_flag = tmem_holder + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = emmy::cluster_ctarank();
 
     if (threadIdx.x == 64) {
         for (int s = 0; s < STAGES; ++s) {
-            emmy::mbar_init(&full[s], 1);
+            emmy::mbar_init(&full[s], LAYOUT == kMM ? 2 : 1);  // dw: one arrival for each CTA
             emmy::mbar_init(&empty[s], 1);
-            emmy::mbar_init(&tail_peer[s], 1);
+            emmy::mbar_init(&tail[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
             emmy::mbar_init(&tfull[a], 1);
             emmy::mbar_init(&tempty[a], 2 * Cfg::kOut);
         }
         emmy::mbar_init(drain, 1);
-        emmy::mbar_init(tail, 1);
         *abort_flag = 0u;
         emmy::fence_barrier_init();
     }
@@ -991,11 +972,10 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
 
     if (warp == 0) {
         // ---------------- loads (both CTAs; completion counted on the leader's barrier)
-        uint32_t stage = 0, phase = 0, tails = 0;
-        uint32_t peer_parity = 0u;  // of tail_peer, one bit for each stage
-        uint32_t issued = 0u, parity_bits = 0u;
+        uint32_t stage = 0, phase = 0;
+        uint32_t issued = 0u, parity_bits = 0u, tail_issued = 0u, tail_uses = 0u;
         bool ok = true;
-        const uint32_t leader_full = emmy::mapa(&full[0], 0), own_tail = emmy::mapa(tail, rank);
+        const uint32_t leader_full = emmy::mapa(&full[0], 0), own_tail = emmy::mapa(&tail[0], rank);
         // One block's loads, completing on the barrier at cluster address `bar`; one thread.
         auto load = [&](const Tile &w, int kb, uint32_t bar) {
             uint8_t *a = sA + stage * kStageA, *b = sB + stage * Cfg::kStageB;
@@ -1015,75 +995,45 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
                 emmy::tma_load_2d_pair(b, &tm_b, bar, k0, w.begin + c0);
             }
         };
-        auto next = [&]() {
-            if (++stage == STAGES) {
-                stage = 0;
-                phase ^= 1u;
-            }
-        };
         for (int t = pair; t < total && ok; t += npairs) {
             const Tile w = tile(t);
-            const int whole = LAYOUT == kMM ? w.kend / BK : w.kb1;
             if (lane == 0) {
-                for (int kb = 0; kb < whole; ++kb) {
+                for (int kb = 0; kb < w.kb1; ++kb) {
                     if (!emmy::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)) {
                         ok = false;
                         break;
                     }
-                    if (rank == 0) {
-                        emmy::mbar_arrive_expect_tx(&full[stage], 2u * Cfg::kStage);
-                        issued |= 1u << stage;
-                        parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
+                    if (LAYOUT == kMM && w.kend - kb * BK < BK) {
+                        // ends inside: the tail warp passes it on
+                        emmy::mbar_arrive_expect_tx(&tail[stage], Cfg::kStage);
+                        load(w, kb, own_tail + stage * 8u);
+                        tail_issued |= 1u << stage;
+                        tail_uses ^= 1u << stage;
+                    } else {
+                        if (rank == 0) {
+                            emmy::mbar_arrive_expect_tx(&full[stage], 2u * Cfg::kStage);
+                            if (LAYOUT == kMM) emmy::mbar_arrive(&full[stage]);
+                            issued |= 1u << stage;
+                            parity_bits = (parity_bits & ~(1u << stage)) | (phase << stage);
+                        }
+                        load(w, kb, leader_full + stage * 8u);
                     }
-                    load(w, kb, leader_full + stage * 8u);
-                    next();
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
                 }
             }
             ok = __all_sync(0xffffffffu, ok);
-            if constexpr (LAYOUT == kMM) {
-                // A last block that ends inside: later rows belong to the next group (or hold
-                // anything), and what the last MMA takes of them becomes zero in both operands
-                // before the leader's barrier completes.  The whole warp does that.
-                if (!ok) break;
-                stage = __shfl_sync(0xffffffffu, stage, 0);
-                phase = __shfl_sync(0xffffffffu, phase, 0);
-                if (whole == w.kb1) continue;
-                ok = emmy::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) {
-                    emmy::mbar_arrive_expect_tx(tail, Cfg::kStage);
-                    load(w, whole, own_tail);
-                }
-                __syncwarp();
-                ok = emmy::mbar_wait_cluster(tail, tails & 1u, abort_flag, EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                ++tails;
-                const int have = w.kend - whole * BK, upto = (have + 15) / 16 * 16;
-                for (int j = 0; j < 2; ++j) zero_panel_rows(sA + stage * kStageA + j * kPanel, have, upto, lane);
-                for (int j = 0; j < CN / 64; ++j)
-                    zero_panel_rows(sB + stage * Cfg::kStageB + j * kPanel, have, upto, lane);
-                emmy::fence_proxy_async();
-                __syncwarp();
-                if (rank == 1) {
-                    if (lane == 0) emmy::mbar_arrive_cluster(emmy::mapa(&tail_peer[stage], 0));
-                } else {
-                    ok = emmy::mbar_wait_cluster(&tail_peer[stage], peer_parity >> stage & 1u, abort_flag,
-                                                 EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    peer_parity ^= 1u << stage;
-                    if (lane == 0) emmy::mbar_arrive(&full[stage]);
-                }
-                next();
-            }
         }
-        if (!ok && rank == 0 && lane == 0) {
+        if (!ok && lane == 0) {
             // loads still in flight land before the pair leaves (bounded)
             volatile uint32_t never = 0u;
-            for (int s = 0; s < STAGES; ++s)
+            for (int s = 0; s < STAGES; ++s) {
                 if (issued & (1u << s)) emmy::mbar_wait_cluster(&full[s], (parity_bits >> s) & 1u, &never, 0u, 20000000ull);
+                if (tail_issued & (1u << s))
+                    emmy::mbar_wait_cluster(&tail[s], (tail_uses >> s & 1u) ^ 1u, &never, 0u, 20000000ull);
+            }
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -1121,12 +1071,34 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
             issue.commit(drain);
         }
         __syncwarp();
+    } else if (LAYOUT == kMM && warp == 2 + Cfg::kOut) {
+        // ---------------- blocks that end inside (both CTAs): the rows behind the end belong to the
+        // next group, or hold anything.  What the last MMA takes of them becomes zero in both
+        // operands before the leader's barrier completes, while the loads run on.
+        uint32_t blocks = 0, tail_parity = 0u;  // of `tail`, one bit for each stage
+        for (int t = pair; t < total; t += npairs) {
+            const Tile w = tile(t);
+            blocks += w.kb1;
+            const int have = w.kend % BK;
+            if (have == 0) continue;
+            const uint32_t stage = (blocks - 1) % STAGES;
+            if (!__all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tail[stage], tail_parity >> stage & 1u, abort_flag,
+                                                                 EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)))
+                break;
+            tail_parity ^= 1u << stage;
+            const int upto = (have + 15) / 16 * 16;
+            for (int j = 0; j < 2; ++j) zero_panel_rows(sA + stage * kStageA + j * kPanel, have, upto, lane);
+            for (int j = 0; j < CN / 64; ++j) zero_panel_rows(sB + stage * Cfg::kStageB + j * kPanel, have, upto, lane);
+            emmy::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) emmy::mbar_arrive_cluster(emmy::mapa(&full[stage], 0));
+        }
+        __syncwarp();
     } else {
         // ---------------- output (both CTAs): own 128 channels of the tile
         const int q = warp & 3, part = (warp - 2) >> 2;
         constexpr int SPAN = BN / (Cfg::kOut / 4);
         const uint32_t leader_tempty = emmy::mapa(&tempty[0], 0);
-        const CUtensorMap *out_map = flags.tma_out ? &tm_out : nullptr;
         uint32_t it = 0;
         for (int t = pair; t < total; t += npairs, ++it) {
             const Tile w = tile(t);
@@ -1137,14 +1109,12 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads, 1)
                                                                  EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)))
                 break;
             emmy::tc_fence_after();
-            store_tile<I8>(p, out_map, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
+            store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
                            part * SPAN, min((part + 1) * SPAN, w.cols), ch, xs, sStore + (warp - 2) * kStoreBytes, lane);
             emmy::tc_fence_before();
             __syncwarp();
             if (lane == 0) emmy::mbar_arrive_cluster(leader_tempty + acc * 8u);
         }
-        if (lane == 0) emmy::tma_store_wait();  // before the shared memory they read from goes
-        __syncwarp();
     }
     emmy::tc_fence_before();
     __syncthreads();
