@@ -52,7 +52,7 @@ namespace {
 //   one FMA gives exactly, tells the side.
 
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
-constexpr float kNearHalf = 0.4999f;
+constexpr float kNearHalf = 0.49999f;  // below: off by less than 127.5 * 2^-24 = 7.6e-6
 
 // x / s to the nearest integer, exact ties to even, for the quotient of the two f32 values.
 __device__ __noinline__ int quantize_exact(float x, float s, float inv) {
@@ -144,11 +144,12 @@ struct Pack {
 // GROUP threads for each row, PER packs of it in each thread's registers; what a longer row has
 // beyond them is read again from L2.
 template <typename T, int VEC, int GROUP, int PER>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride,
+__global__ void __launch_bounds__(GROUP == 32 ? 256 : GROUP) quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride,
                                                             int8_t *__restrict__ q, int64_t q_stride,
                                                             float *__restrict__ scale, int64_t rows, int64_t k) {
+    constexpr int THREADS = GROUP == 32 ? 256 : GROUP;
     const int tid = threadIdx.x % GROUP;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / GROUP) + threadIdx.x / GROUP;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * (THREADS / GROUP) + threadIdx.x / GROUP;
     const bool live = r < rows;
     emmy::wait_for_prior_grid();
     emmy::let_next_grid_start();
@@ -169,10 +170,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T *__restrict_
     }
     peak = __reduce_max_sync(0xffffffffu, peak);
     if constexpr (GROUP > 32) {
-        __shared__ uint32_t s_peak[8];
+        __shared__ uint32_t s_peak[GROUP / 32];
         if ((threadIdx.x & 31) == 0) s_peak[threadIdx.x >> 5] = peak;
         __syncthreads();
-        peak = __reduce_max_sync(0xffffffffu, s_peak[threadIdx.x & 7]);
+        peak = __reduce_max_sync(0xffffffffu, s_peak[threadIdx.x % (GROUP / 32)]);
     }
     if (!live) return;
     const bool bad = peak >= Bits<T>::kInf;
@@ -427,12 +428,12 @@ int launch_product(const Call &call, Product p, bool bf16) {
         return per_sm * (cluster <= 2 ? kSms : cluster == 4 ? 132 : 120);
     };
     // Idle SMs take parts of the sums, as long as a part is worth the exchange: 4 blocks of it for
-    // the few columns of a narrow tile, 16 for a wide one (1022 rows, 8 experts, dx [1000, 776], 13
+    // the few columns of a narrow tile, 8 and 16 for wider ones (1022 rows, 8 experts, dx [1000, 776], 13
     // blocks: 11 us whole, 18 in halves; 60000 rows, dw [256, 256]: 275 us whole, 42 in eighths).
     int split = 1;
     if (!pair)
         while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident(split * 2) &&
-               kblocks >= split * 2 * (bn <= 32 ? 4 : 16))
+               kblocks >= split * 2 * (bn <= 32 ? 4 : bn == 64 ? 8 : 16))
             split *= 2;
     const int cluster = pair ? 2 : split;
     int64_t clusters = pair ? most(2 * kTileM, pair) : most(kTileM, bn);
@@ -456,7 +457,7 @@ int run_product(const char *name, int dev, int operands, const Product &p, uint6
     return operands == kS8 ? launch_product<true>(call, p, false) : launch_product<false>(call, p, operands == EMMY_BF16);
 }
 
-// A warp for each row while its registers hold the row, else the whole block.
+// A warp for each row while its registers hold the row, else a block of 128 or 256 threads.
 template <typename T>
 int launch_quantize(const Call &call, const T *x, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
                     int64_t rows, int64_t k) {
@@ -464,14 +465,21 @@ int launch_quantize(const Call &call, const T *x, int64_t x_stride, int8_t *q, i
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && reinterpret_cast<uintptr_t>(q) % VEC == 0 &&
                      x_stride % VEC == 0 && q_stride % VEC == 0 && k % VEC == 0;
     auto go = [&](auto kernel, int group) {
-        cudaLaunchConfig_t cfg = config(call, ceil_div(rows, 256 / group), 256, 0);
+        const int threads = group == 32 ? 256 : group;
+        cudaLaunchConfig_t cfg = config(call, ceil_div(rows, threads / group), threads, 0);
         cudaLaunchAttribute attr = early_start();
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         return launched(call, cudaLaunchKernelEx(&cfg, kernel, x, x_stride, q, q_stride, scale, rows, k));
     };
-    if (vec) return k <= 32 * 4 * VEC ? go(quantize_rows_kernel<T, VEC, 32, 4>, 32) : go(quantize_rows_kernel<T, VEC, 256, 4>, 256);
-    return k <= 32 * 16 ? go(quantize_rows_kernel<T, 1, 32, 16>, 32) : go(quantize_rows_kernel<T, 1, 256, 16>, 256);
+    if (vec) {
+        if (k <= 32 * 4 * VEC) return go(quantize_rows_kernel<T, VEC, 32, 4>, 32);
+        if (k <= 128 * 4 * VEC) return go(quantize_rows_kernel<T, VEC, 128, 4>, 128);
+        return go(quantize_rows_kernel<T, VEC, 256, 4>, 256);
+    }
+    if (k <= 32 * 32) return go(quantize_rows_kernel<T, 1, 32, 32>, 32);
+    if (k <= 128 * 32) return go(quantize_rows_kernel<T, 1, 128, 32>, 128);
+    return go(quantize_rows_kernel<T, 1, 256, 32>, 256);
 }
 
 int check_common(const char *name, int dev, int64_t rows, int64_t experts, int64_t n, int64_t k) {

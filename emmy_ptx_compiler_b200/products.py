@@ -54,24 +54,31 @@ class BoundProduct:
             runtime._check(rc)
 
 
+_dtype_names: dict = {}
+
+
 def _dtype(t) -> str:
-    return str(t.dtype).rpartition(".")[2]
+    name = _dtype_names.get(t.dtype)
+    if name is None:
+        name = _dtype_names[t.dtype] = str(t.dtype).rpartition(".")[2]
+    return name
 
 
 def _matrix(name: str, t, shape: tuple, dtypes: tuple) -> int:
     """Check a tensor's shape (None: any extent), dtype and contiguous innermost axis; its row stride."""
-    if len(t.shape) != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
+    have = tuple(t.shape)
+    if have != shape and (len(have) != len(shape) or any(w is not None and h != w for h, w in zip(have, shape))):
         want = ", ".join("any" if s is None else str(s) for s in shape)
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({want})")
+        raise ValueError(f"{name} has shape {have}, expected ({want})")
     if _dtype(t) not in dtypes:
         raise ValueError(f"{name} is {_dtype(t)}, expected {' or '.join(dtypes)}")
     stride = t.stride()
-    if t.shape[-1] > 1 and stride[-1] != 1:
+    if have[-1] > 1 and stride[-1] != 1:
         raise ValueError(f"{name}'s innermost axis must be contiguous, its stride is {stride[-1]}")
     if len(shape) == 1:
         return 1
     # a single row has no stride to speak of; report one that any check accepts
-    return stride[-2] if t.shape[-2] > 1 else max(stride[-2], t.shape[-1])
+    return stride[-2] if have[-2] > 1 else max(stride[-2], have[-1])
 
 
 def _rows_apart(name: str, t, row_stride: int) -> None:
