@@ -48,8 +48,10 @@ namespace {
 // * fma(x, 1 / s, 1.5 * 2^23) rounds the exact product to an integer, ties to even, and leaves
 //   that integer in the low byte of the result's bits;
 // * 1 / s is off by half a step, so below 128 the product is off by less than 1e-5 and decides
-//   every quotient but those that close to a half.  For these the sign of x - (q +- 1/2) s, which
-//   one FMA gives exactly, tells the side.
+//   every quotient but those that close to a half (16-bit rows meet exact halves often: a row whose
+//   peak is a power of two has one in a few hundred values).  For these the residual x - q s tells:
+//   it is a multiple of half a step of s and at most about s / 2, so the FMA that computes it is
+//   exact, and comparing it with s / 2 settles the side and the ties.
 
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
 constexpr float kNearHalf = 0.49999f;  // below: off by less than 127.5 * 2^-24 = 7.6e-6
@@ -115,16 +117,25 @@ struct Pack {
     // exact: every value goes the long way (a scale so small that its reciprocal needs lifting)
     __device__ __forceinline__ void store(int8_t *q, float s, float inv, float lift, bool zero, bool exact) const {
         uint32_t r[VEC];
-        float near = exact ? 1.0f : 0.0f;
+        float near = 0.0f;
         #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const float x = Bits<T>::value(v[i]), f = fmaf(x, inv, kRoundMagic);
             r[i] = __float_as_uint(f);
             near = fmaxf(near, fabsf(fmaf(x, inv, kRoundMagic - f)));
         }
-        if (near > kNearHalf) {
+        if (exact) {
             #pragma unroll
             for (int i = 0; i < VEC; ++i) r[i] = static_cast<uint32_t>(quantize_exact(Bits<T>::value(v[i]) * lift, s, inv));
+        } else if (near > kNearHalf) {
+            const uint32_t half = __float_as_uint(0.5f * s);
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float rest = fmaf(kRoundMagic - __uint_as_float(r[i]), s, Bits<T>::value(v[i]));
+                const uint32_t bits = __float_as_uint(rest);
+                // beyond the half, or on it beside an odd integer: one further
+                if ((bits & 0x7fffffffu) + (r[i] & 1u) > half) r[i] += 1u | static_cast<uint32_t>(static_cast<int>(bits) >> 31);
+            }
         }
         if constexpr (VEC == 1) {
             *q = zero ? 0 : static_cast<int8_t>(r[0]);
@@ -475,7 +486,8 @@ int launch_quantize(const Call &call, const T *x, int64_t x_stride, int8_t *q, i
     if (vec) {
         if (k <= 32 * 4 * VEC) return go(quantize_rows_kernel<T, VEC, 32, 4>, 32);
         if (k <= 128 * 4 * VEC) return go(quantize_rows_kernel<T, VEC, 128, 4>, 128);
-        return go(quantize_rows_kernel<T, VEC, 256, 4>, 256);
+        if (k <= 256 * 4 * VEC) return go(quantize_rows_kernel<T, VEC, 256, 4>, 256);
+        return go(quantize_rows_kernel<T, VEC, 256, 8>, 256);
     }
     if (k <= 32 * 32) return go(quantize_rows_kernel<T, 1, 32, 32>, 32);
     if (k <= 128 * 32) return go(quantize_rows_kernel<T, 1, 128, 32>, 128);
