@@ -216,13 +216,15 @@ int report(int code, const char *fmt, ...) {
     return emmy_record_error(code, buf);
 }
 
-// The call's device, made current for the launch and put back afterwards.
+// The call's device, made current for the launch and put back afterwards.  It is set even where it
+// is the thread's device already: a thread that has not used it yet has no context, which encoding
+// a tensor map needs.
 struct DeviceScope {
     int prev = -1;
     cudaError_t err;
     explicit DeviceScope(int dev) {
         err = cudaGetDevice(&prev);
-        if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev);
+        if (err == cudaSuccess) err = cudaSetDevice(dev);
         if (prev == dev) prev = -1;
     }
     ~DeviceScope() {
@@ -230,7 +232,8 @@ struct DeviceScope {
     }
 };
 
-constexpr int64_t kMaxExtent = (1ll << 31) - 1;
+constexpr int64_t kMaxExtent = (1ll << 31) - 1024;  // 32-bit extents, with room to round them up to tiles
+constexpr int64_t kMaxTiles = 1ll << 30;
 
 bool bad_extent(int64_t v) { return v < 0 || v > kMaxExtent; }
 
@@ -422,8 +425,8 @@ int launch_product(const Call &call, Product p, bool bf16) {
         if (cext > 128 && tiles(256, 256) >= kSms / 4) pair = 256;
         else if (tiles(256, 128) >= kSms / 4) pair = 128;
     }
-    if (most(kTileM, p.dw ? 64 : 16) > kMaxExtent)
-        return report(EMMY_ERR_INVALID, "%s: an output of more than 2^31 tiles is not supported", call.name);
+    if (most(kTileM, p.dw ? 64 : 16) > kMaxTiles)
+        return report(EMMY_ERR_INVALID, "%s: an output of more than 2^30 tiles is not supported", call.name);
     const int bn = pair ? pair : p.dw ? 128 : !tma ? (even <= 24 ? 32 : 128) : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
 
     CUtensorMap ta{}, tb{};
@@ -497,7 +500,7 @@ int launch_quantize(const Call &call, const T *x, int64_t x_stride, int8_t *q, i
 int check_common(const char *name, int dev, int64_t rows, int64_t experts, int64_t n, int64_t k) {
     if (dev < 0 || dev >= 64) return report(EMMY_ERR_INVALID, "%s: bad device %d", name, dev);
     if (bad_extent(rows) || bad_extent(n) || bad_extent(k))
-        return report(EMMY_ERR_INVALID, "%s: rows, n and k must be within 0 and 2^31 - 1", name);
+        return report(EMMY_ERR_INVALID, "%s: rows, n and k must be within 0 and 2^31 - 1024", name);
     if (experts < 0 || experts > kMaxExperts)
         return report(EMMY_ERR_INVALID, "%s: experts must be within 0 and %d", name, kMaxExperts);
     return EMMY_OK;

@@ -205,7 +205,7 @@ int emmy_sum_f32_noalloc(int dev, const float *x, uint64_t n, float *out, uint64
  * `stream`, allocate nothing, keep no state between calls and never
  * synchronise, so they can be recorded into graphs and overlap each other.
  * Extents and strides are counted in elements; an innermost stride not given
- * is 1.  Outputs must not overlap inputs.  Extents of 0 are fine.
+ * is 1.  Outputs must not overlap inputs.  Extents go from 0 to 2^31 - 1024.
  *
  * Groups: `offsets` (device, experts + 1 words) names expert e's rows
  * [offsets[e], offsets[e + 1]).  Rows outside every group are neither used

@@ -490,3 +490,198 @@ def test_more_experts_than_any_tile_has_lanes():
     want = torch.zeros(e, n, k, dtype=torch.float64, device="cuda").index_add_(0, owner, outer)
     size = torch.zeros_like(want).index_add_(0, owner, outer.abs())
     _close(dw, want, size, 4)
+
+
+NAN_PADS = [([3, 20, 0, 9], 200, 72), ([3, 20, 0, 9], 136, 101), ([150, 40, 260], 1000, 100), ([300] * 8, 1544, 1000)]
+
+
+@pytest.mark.parametrize("counts,n,k", NAN_PADS)
+def test_what_lies_between_rows_is_never_used(counts, n, k):
+    """Rows padded with NaN, in every operand of all three products and of the 8-bit one."""
+    g = _gen(21)
+    rows, e, pad = sum(counts), len(counts), 8
+    x, dy = _padded(rows, k, BF16, g, pad), _padded(rows, n, BF16, g, pad)
+    w = _padded(e * n, k, BF16, g, pad, std=0.1)
+    for t, cols in ((x, k), (dy, n), (w, k)):
+        t.as_strided((t.shape[0], pad), (cols + pad, 1), t.storage_offset() + cols).fill_(float("nan"))
+    w = w.unflatten(0, (e, n))
+    off = _offsets(counts)
+    out = torch.empty(rows, n, dtype=BF16, device="cuda")
+    dx = torch.empty(rows, k, dtype=BF16, device="cuda")
+    dw = torch.empty(e, n, k, dtype=F32, device="cuda")
+    products.grouped_matmul(x, w, off, out, stream=_stream())
+    products.grouped_matmul(dy, w.transpose(1, 2), off, dx, stream=_stream())
+    products.grouped_matmul_dw(dy, x, off, dw, stream=_stream())
+    assert out.isfinite().all() and dx.isfinite().all() and dw.isfinite().all()
+    at = 0
+    for i, c in enumerate(counts):
+        X, D, W = x[at:at + c].double(), dy[at:at + c].double(), w[i].double()
+        _close(out[at:at + c], X @ W.t(), X.abs() @ W.abs().t(), k)
+        _close(dx[at:at + c], D @ W, D.abs() @ W.abs(), n)
+        _close(dw[i], D.t() @ X, D.abs().t() @ X.abs(), c)
+        at += c
+
+
+def test_broadcast_rows_and_shared_weights():
+    """Strides of 0: one row for all rows of x, one matrix for all experts."""
+    g = _gen(22)
+    counts, n, k = [4, 0, 70, 6], 264, 128
+    rows, e = sum(counts), len(counts)
+    x = _padded(1, k, F16, g).expand(rows, k)
+    w = _padded(n, k, F16, g).unsqueeze(0).expand(e, n, k)
+    off = _offsets(counts)
+    out = torch.empty(rows, n, dtype=F32, device="cuda")
+    products.grouped_matmul(x, w, off, out, stream=_stream())
+    _close(out, x.double() @ w[0].double().t(), x.double().abs() @ w[0].double().abs().t(), k)
+    dw = torch.empty(e, n, k, dtype=F32, device="cuda")
+    dy = _padded(rows, n, F16, g)
+    products.grouped_matmul_dw(dy, x, off, dw, stream=_stream())
+    for i, (a, b) in enumerate(zip(off.tolist(), off.tolist()[1:])):
+        d, X = dy[a:b].double(), x[a:b].double()
+        _close(dw[i], d.t() @ X, d.abs().t() @ X.abs(), b - a)
+
+
+def test_weights_in_the_other_order_and_single_axes():
+    """[experts, k, n] weights as a view, and extents of 1, whose strides mean nothing."""
+    g = _gen(23)
+    for n, k in ((96, 64), (1, 64), (96, 1), (1, 1)):
+        w = _padded(3 * k, n, BF16, g).unflatten(0, (3, k)).transpose(1, 2)
+        x = _padded(9, k, BF16, g)
+        off, out = _offsets([2, 0, 7]), torch.empty(9, n, dtype=F32, device="cuda")
+        products.grouped_matmul(x, w, off, out, stream=_stream())
+        for i, (a, b) in enumerate(((0, 2), (2, 2), (2, 9))):
+            X, W = x[a:b].double(), w[i].double()
+            _close(out[a:b], X @ W.t(), X.abs() @ W.abs().t(), k)
+
+
+@pytest.mark.parametrize("k", [2048, 2041])
+def test_positions_beyond_31_bits(k):
+    """Operands and outputs of more than 2^31 values: the last rows' addresses need 64 bits."""
+    rows, n = 1_100_000, 2048
+    x = torch.zeros(rows, k, dtype=torch.int8, device="cuda")
+    tail = 300
+    g = _gen(24)
+    x[-tail:] = torch.randint(-127, 128, (tail, k), dtype=torch.int8, device="cuda", generator=g)
+    w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda", generator=g)
+    xs, ws = torch.ones(rows, device="cuda"), torch.ones(n, device="cuda")
+    out = torch.empty(rows, n, dtype=F32, device="cuda")
+    assert x.numel() > 1 << 31 and out.numel() > 1 << 31
+    products.int8_matmul(x, xs, w, ws, out, stream=_stream())
+    assert torch.equal(out[-tail:], (x[-tail:].double() @ w.double().t()).float())
+    assert (out[:100] == 0).all() and (out[-tail - 100:-tail] == 0).all()
+
+
+def test_experts_beyond_31_bits():
+    """Weights and their gradients of more than 2^31 values."""
+    g = _gen(25)
+    e, n, k = 600, 2048, 2048
+    counts = [0] * (e - 2) + [5, 11]
+    w = torch.empty(e, n, k, dtype=BF16, device="cuda")
+    assert w.numel() > 1 << 31
+    w[-2:].normal_(generator=g)
+    x, dy = _padded(16, k, BF16, g), _padded(16, n, BF16, g)
+    off = _offsets(counts)
+    out = torch.empty(16, n, dtype=F32, device="cuda")
+    products.grouped_matmul(x, w, off, out, stream=_stream())
+    for i, a, b in ((-2, 0, 5), (-1, 5, 16)):
+        X, W = x[a:b].double(), w[i].double()
+        _close(out[a:b], X @ W.t(), X.abs() @ W.abs().t(), k)
+    products.grouped_matmul_dw(dy, x, off, w, stream=_stream())
+    for i, a, b in ((-2, 0, 5), (-1, 5, 16)):
+        D, X = dy[a:b].double(), x[a:b].double()
+        _close(w[i], D.t() @ X, D.abs().t() @ X.abs(), b - a)
+    assert (w[:2] == 0).all() and (w[-4:-2] == 0).all()
+
+
+def test_long_sums_are_split_and_joined_in_order():
+    """Few tiles and long sums: parts of them on several SMs, with the same bits every time."""
+    g = _gen(26)
+    off = _offsets([20011, 0])
+    dy, x = _padded(20011, 264, BF16, g), _padded(20011, 200, BF16, g)
+    dws = [torch.empty(2, 264, 200, dtype=F32, device="cuda") for _ in range(3)]
+    for dw in dws:
+        products.grouped_matmul_dw(dy, x, off, dw, stream=_stream())
+    D, X = dy.double(), x.double()
+    _close(dws[0][0], D.t() @ X, D.abs().t() @ X.abs(), 20011)
+    assert torch.equal(dws[0], dws[1]) and torch.equal(dws[0], dws[2]) and (dws[0][1] == 0).all()
+    for rows in (1, 9, 20, 40, 100):
+        xq = torch.randint(-127, 128, (rows, 16384), dtype=torch.int8, device="cuda", generator=g)
+        wq = torch.randint(-127, 128, (300, 16384), dtype=torch.int8, device="cuda", generator=g)
+        ones = torch.ones(300, device="cuda")
+        out = torch.empty(rows, 300, device="cuda")
+        products.int8_matmul(xq, ones[:rows], wq, ones, out, stream=_stream())
+        assert torch.equal(out, (xq.double() @ wq.double().t()).float())
+        xb, wb = _padded(rows, 8192, F16, g), _padded(300, 8192, F16, g).unsqueeze(0)
+        outs = [torch.empty(rows, 300, dtype=F16, device="cuda") for _ in range(2)]
+        for o in outs:
+            products.grouped_matmul(xb, wb, _offsets([rows]), o, stream=_stream())
+        _close(outs[0], xb.double() @ wb[0].double().t(), xb.double().abs() @ wb[0].double().abs().t(), 8192)
+        assert torch.equal(outs[0], outs[1])
+
+
+FIRST_CALL_RECORDED = """
+import torch
+from emmy_ptx_compiler_b200 import products, runtime
+runtime.init(0)
+rows, n, k, e = 40, 256, 512, 2
+x = torch.randint(-3, 4, (rows, k), device="cuda").to(torch.bfloat16)
+w = torch.randint(-3, 4, (e, n, k), device="cuda").to(torch.bfloat16)
+off = torch.tensor([0, 30, 40], dtype=torch.int32, device="cuda")
+out = torch.zeros(rows, n, device="cuda")
+q, s = torch.zeros(rows, k, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+with runtime.Graph.record(0, side.cuda_stream) as graph:
+    runtime._check(runtime.lib().emmy_memset_d8(0, out.data_ptr(), 1, out.numel() * 4, side.cuda_stream))
+    products.grouped_matmul(x, w, off, out, stream=side.cuda_stream)
+    products.quantize_rows(x, q, s, stream=side.cuda_stream)
+graph.launch(side.cuda_stream)
+torch.cuda.synchronize()
+want = torch.cat([x[:30].double() @ w[0].double().t(), x[30:].double() @ w[1].double().t()])
+assert torch.equal(out.double(), want)
+assert torch.equal(s, (x.abs().amax(1).double() / 127).float())
+assert products.status(0) == 0
+graph.close()
+print("recorded")
+"""
+
+
+def test_a_first_call_can_be_recorded(cuda_device):
+    """In a process that has made no call before: loading the kernels does not disturb the recording."""
+    import subprocess
+    import sys
+
+    from conftest import REPO
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_RECORDED], cwd=REPO, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "recorded" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_host_threads_at_once():
+    """Calls from two threads on their own streams: nothing on the host side is shared either."""
+    import threading
+
+    g = _gen(27)
+    counts, n, k = [33, 0, 80], 256, 264
+    rows, e = sum(counts), len(counts)
+    x, w = _padded(rows, k, F16, g), _padded(e * n, k, F16, g).unflatten(0, (e, n))
+    off = _offsets(counts)
+    want = torch.empty(rows, n, dtype=F16, device="cuda")
+    products.grouped_matmul(x, w, off, want, stream=_stream())
+    torch.cuda.synchronize()
+    outs = [torch.empty_like(want) for _ in range(2)]
+    errors = []
+
+    def run(o):
+        try:
+            s = torch.cuda.Stream()
+            for _ in range(50):
+                products.grouped_matmul(x, w, off, o, stream=s.cuda_stream)
+            s.synchronize()
+        except Exception as exc:  # reported below, on the test's thread
+            errors.append(exc)
+
+    threads = [threading.Thread(target=run, args=(o,)) for o in outs]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors and torch.equal(outs[0], want) and torch.equal(outs[1], want)
