@@ -529,11 +529,23 @@ struct TcConfig {
     static constexpr uint32_t kTmemCols = BN >= 64 ? 4 * BN : 2 * BN;
 };
 
-// Warp 0 loads operand tiles by TMA (TMA false: the last 16 warps load those operands whose rows
-// TMA cannot take), warp 1 issues the MMAs into one of two accumulators, the warps from 2 on
-// turn the other into output, 4 or 8 of them: a warp reaches 32 of the 128 lanes.  In a cluster of several CTAs every CTA sums its part of k, and the parts are
-// added in rank order: each CTA finishes its share of the columns, for which the others send their
-// parts through distributed shared memory.  The result depends on neither timing nor the number of SMs.
+// One CTA on 128 channels x BN rows of output.  Warp 0 loads operand tiles by TMA (TMA false: the
+// last warps load those operands whose rows TMA cannot take), warp 1 issues the MMAs into one of two
+// accumulators, the warps from 2 on turn the other into output, 4 or 8 of them: a warp reaches 32 of
+// the 128 lanes.
+//
+// With BN of 16 or 32, for groups of a few rows, this is bound by reading the weights: 64 experts
+// [2048, 4096] for 512 rows take 168 us, 6.4 TB/s.  Two CTAs share an SM, so that one's loads cover
+// the other's start and end.  Where there are fewer tiles than SMs a cluster of CTAs divides each
+// sum: one token of 8 experts [1024, 2048] takes 10 us in quarters against 13 undivided.  Each CTA
+// sums its part of k and the parts are added in rank order: a CTA finishes its share of the
+// columns, for which the others send their parts through distributed shared memory, so the result
+// depends on no timing.
+//
+// Tensor memory is held from start to end, and the CTAs of a cluster wait for each other.  Two
+// kernels that did so with more than 512 columns between them on one SM could block each other;
+// the CTAs here and those of the attention and GEMM families that take more than a few columns also
+// take more than half of an SM's shared memory, so no SM holds two of them.
 template <bool I8, int LAYOUT, int BN, bool TMA>
 __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, BN, TMA>::kPerSm)
     product_tc_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
@@ -893,7 +905,14 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
 // 128 channels of A and its half of B's rows, the leader issues cta_group::2 MMAs over both CTAs'
 // shared memory, and each CTA turns its own 128 lanes into output while the next tile accumulates.
 // A pair moves 64 bytes into shared memory per SM and clock of MMA (BN = 256), half of what a
-// single CTA's 128 x 128 tile needs - more than L2 delivers.
+// single CTA's 128 x 128 tile needs.
+//
+// Bound by the tensor cores where sums are long: 16384 rows, 4 experts [4096, 4096], take 345 us (1.59
+// PFLOP/s bf16), int8 8192^3 takes 318 us (3.46 POP/s).  Sums of a few blocks are bound by the way
+// out (a 32 x 32 piece of a tile takes its warp 800 cycles): 8192 rows, 32 experts, dx [1024, 512] 20 us.
+// Measured on the way: 6 stages against 4, 352 against 382 us for the first of these; MMAs issued
+// from a branch of one lane, with their operands moved to uniform registers one by one, 590 cycles a
+// block against 512 of MMA.
 
 template <int BN>
 struct PairConfig {
