@@ -57,8 +57,9 @@ namespace {
 //   it is a multiple of half a step of s and at most about s / 2, so the FMA that computes it is
 //   exact, and comparing it with s / 2 settles the side and the ties.
 //
-// 16381 x 8192 bf16 rows take 75 to 83 us (4.9 to 5.4 TB/s; the more of their quotients lie near a
-// half, the longer), f32 rows 121 us (5.5 TB/s), one row 2 us.
+// 16381 x 8192 f32 rows take 106 us (6.3 TB/s), bf16 rows 75 to 82 us (4.9 to 5.4 TB/s), which issue
+// instructions in 7 of 10 cycles: the more of their quotients lie near a half, the longer.  One row
+// takes 2 us.
 
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
 constexpr float kNearHalf = 0.49999f;  // below: off by less than 127.5 * 2^-24 = 7.6e-6
@@ -124,22 +125,22 @@ struct Pack {
     // exact: every value goes the long way (a scale so small that its reciprocal needs lifting)
     __device__ __forceinline__ void store(int8_t *q, float s, float inv, float lift, bool zero, bool exact) const {
         uint32_t r[VEC];
-        float near = 0.0f;
+        float rest[VEC], near = 0.0f;
         #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const float x = Bits<T>::value(v[i]), f = fmaf(x, inv, kRoundMagic);
             r[i] = __float_as_uint(f);
-            near = fmaxf(near, fabsf(fmaf(x, inv, kRoundMagic - f)));
+            rest[i] = fmaf(kRoundMagic - f, s, x);
+            near = fmaxf(near, fabsf(rest[i]));
         }
         if (exact) {
             #pragma unroll
             for (int i = 0; i < VEC; ++i) r[i] = static_cast<uint32_t>(quantize_exact(Bits<T>::value(v[i]) * lift, s, inv));
-        } else if (near > kNearHalf) {
+        } else if (near > kNearHalf * s) {
             const uint32_t half = __float_as_uint(0.5f * s);
             #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float rest = fmaf(kRoundMagic - __uint_as_float(r[i]), s, Bits<T>::value(v[i]));
-                const uint32_t bits = __float_as_uint(rest);
+                const uint32_t bits = __float_as_uint(rest[i]);
                 // beyond the half, or on it beside an odd integer: one further
                 if ((bits & 0x7fffffffu) + (r[i] & 1u) > half) r[i] += 1u | static_cast<uint32_t>(static_cast<int>(bits) >> 31);
             }
