@@ -435,7 +435,12 @@ int launch_product(const Call &call, Product p, bool bf16) {
     }
     if (most(kTileM, p.dw ? 64 : 16) > kMaxTiles)
         return report(EMMY_ERR_INVALID, "%s: an output of more than 2^30 tiles is not supported", call.name);
-    const int bn = pair ? pair : p.dw ? 128 : !tma ? (even <= 24 ? 32 : 128) : even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 ? 64 : 128;
+    // Output rows of a single CTA's tile: a few more than an even group has, so that an uneven one
+    // still fits; 64 until there are tiles for every SM (300 rows, [512, 1024]: 7.5 against 8.3 us at 128).
+    int bn = 128;
+    if (pair) bn = pair;
+    else if (!p.dw && !tma) bn = even <= 24 ? 32 : 128;
+    else if (!p.dw) bn = even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 || tiles(kTileM, 128) <= kSms ? 64 : 128;
 
     CUtensorMap ta{}, tb{};
     const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
@@ -450,13 +455,13 @@ int launch_product(const Call &call, Product p, bool bf16) {
         return per_sm * (cluster <= 2 ? kSms : cluster == 4 ? 132 : 120);
     };
     // Idle SMs take parts of the sums, as long as a part is worth the exchange: 4 blocks of it for
-    // the few columns of a narrow tile, 8 and 16 for wider ones (1022 rows, 8 experts, dx [1000, 776], 13
-    // blocks: 11 us whole, 18 in halves; 60000 rows, dw [256, 256]: 275 us whole, 42 in eighths).
+    // the few columns of a narrow tile, 8 (of 32 or more) and 16 for wider ones (1022 rows, 8 experts, dx
+    // [1000, 776], 13 blocks at 128 wide: 11 us whole, 18 in halves; 90 rows, [768, 8192]: 11 us in
+    // eighths, 13 in quarters; 60000 rows, dw [256, 256]: 275 us whole, 42 in eighths).
+    const int64_t part = bn <= 32 ? 4 : bn == 64 ? 8 : 16;
     int split = 1;
-    if (!pair)
-        while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident(split * 2) &&
-               kblocks >= split * 2 * (bn <= 32 ? 4 : bn == 64 ? 8 : 16))
-            split *= 2;
+    if (!pair && (bn != 64 || kblocks >= 32))
+        while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident(split * 2) && kblocks >= split * 2 * part) split *= 2;
     const int cluster = pair ? 2 : split;
     int64_t clusters = pair ? most(2 * kTileM, pair) : most(kTileM, bn);
     if (clusters > resident(cluster) / cluster) clusters = resident(cluster) / cluster;
