@@ -143,6 +143,8 @@ __host__ __device__ constexpr uint32_t idesc_s8(uint32_t m, uint32_t n) {
 namespace {
 
 constexpr uint64_t kWaitNs = 2000000000ull;  // per wait: orders of magnitude above any legal one
+// A wait for a whole sum may last as long as its blocks do, at 20 us each (0.3 to 2 us measured).
+__device__ __forceinline__ uint64_t sum_wait_ns(int blocks) { return kWaitNs + static_cast<uint64_t>(blocks) * 20000ull; }
 constexpr int kTileM = 128;
 constexpr uint32_t kBlockBytes = 128;                  // one 128-byte swizzle row of k (or of m, c)
 constexpr uint32_t kPanel = 64 * kBlockBytes;          // 64 k x 64 m (or c) of an MN-major 16-bit operand
@@ -761,7 +763,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                 const Channel ch = channel<I8>(p, w, m);
                 RowScales<I8, (SPAN + 31) / 32> xs(p, w, part * SPAN, lane);
                 ok = __all_sync(0xffffffffu, emmy::mbar_wait(&tfull[acc], aphase, abort_flag,
-                                                             EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs));
+                                                             EMMY_STATUS_TIMEOUT_EPILOGUE, sum_wait_ns(w.kb1 - w.kb0)));
                 if (!ok) break;
                 emmy::tc_fence_after();
                 const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
@@ -1125,7 +1127,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
             const Channel ch = channel<I8>(p, w, w.m0 + q * 32 + lane);
             const RowScales<I8, SPAN / 32> xs(p, w, part * SPAN, lane);
             if (!__all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tfull[acc], aphase, abort_flag,
-                                                                 EMMY_STATUS_TIMEOUT_EPILOGUE, kWaitNs)))
+                                                                 EMMY_STATUS_TIMEOUT_EPILOGUE, sum_wait_ns(w.kb1 - w.kb0))))
                 break;
             emmy::tc_fence_after();
             store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,

@@ -647,15 +647,41 @@ graph.close()
 print("recorded")
 """
 
+FIRST_CALL_IN_A_TORCH_GRAPH = """
+import torch
+from emmy_ptx_compiler_b200 import products
+x = torch.randint(-3, 4, (600, 512), device="cuda").to(torch.float16)
+w = torch.randint(-3, 4, (2, 2560, 512), device="cuda").to(torch.float16)
+off = torch.tensor([0, 250, 600], dtype=torch.int32, device="cuda")
+out, dw = torch.zeros(600, 2560, device="cuda"), torch.zeros(2, 2560, 512, device="cuda")
+dy = torch.randint(-3, 4, (600, 2560), device="cuda").to(torch.float16)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    s = torch.cuda.current_stream().cuda_stream
+    products.grouped_matmul(x, w, off, out, stream=s)
+    products.grouped_matmul_dw(dy, x, off, dw, stream=s)
+    out.mul_(2)
+for _ in range(3):
+    graph.replay()
+torch.cuda.synchronize()
+for e, (a, b) in enumerate(((0, 250), (250, 600))):
+    assert torch.equal(out[a:b].double(), 2 * (x[a:b].double() @ w[e].double().t()))
+    assert torch.equal(dw[e].double(), dy[a:b].double().t() @ x[a:b].double())
+assert products.status(0) == 0
+print("recorded")
+"""
 
-def test_a_first_call_can_be_recorded(cuda_device):
+
+@pytest.mark.parametrize("code", [FIRST_CALL_RECORDED, FIRST_CALL_IN_A_TORCH_GRAPH])
+def test_a_first_call_can_be_recorded(code, cuda_device):
     """In a process that has made no call before: loading the kernels does not disturb the recording."""
     import subprocess
     import sys
 
     from conftest import REPO
 
-    r = subprocess.run([sys.executable, "-c", FIRST_CALL_RECORDED], cwd=REPO, capture_output=True, text=True, timeout=300)
+    r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "recorded" in r.stdout, r.stderr[-2000:]
 
 
