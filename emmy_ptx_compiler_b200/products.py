@@ -43,8 +43,13 @@ class BoundProduct:
     """A launch with its arguments prepared once (the tensors stay alive and must keep their
     storage): each call is one C-ABI launch."""
 
+    _fns: dict = {}
+
     def __init__(self, fn: str, args: tuple, keep: tuple):
-        self._fn = getattr(runtime.lib(), fn)
+        f = self._fns.get(fn)
+        if f is None:
+            f = self._fns[fn] = getattr(runtime.lib(), fn)
+        self._fn = f
         self._args = args
         self._keep = keep
 
@@ -67,18 +72,23 @@ def _dtype(t) -> str:
 def _matrix(name: str, t, shape: tuple, dtypes: tuple) -> int:
     """Check a tensor's shape (None: any extent), dtype and contiguous innermost axis; its row stride."""
     have = tuple(t.shape)
-    if have != shape and (len(have) != len(shape) or any(w is not None and h != w for h, w in zip(have, shape))):
-        want = ", ".join("any" if s is None else str(s) for s in shape)
-        raise ValueError(f"{name} has shape {have}, expected ({want})")
+    if have != shape:
+        fits = len(have) == len(shape)
+        for h, w in zip(have, shape):
+            if w is not None and h != w:
+                fits = False
+        if not fits:
+            want = ", ".join("any" if w is None else str(w) for w in shape)
+            raise ValueError(f"{name} has shape {have}, expected ({want})")
     if _dtype(t) not in dtypes:
         raise ValueError(f"{name} is {_dtype(t)}, expected {' or '.join(dtypes)}")
-    stride = t.stride()
-    if have[-1] > 1 and stride[-1] != 1:
+    stride, cols = t.stride(), have[-1]
+    if cols > 1 and stride[-1] != 1:
         raise ValueError(f"{name}'s innermost axis must be contiguous, its stride is {stride[-1]}")
     if len(shape) == 1:
         return 1
     # a single row has no stride to speak of; report one that any check accepts
-    return stride[-2] if have[-2] > 1 else max(stride[-2], have[-1])
+    return stride[-2] if have[-2] > 1 else max(stride[-2], cols)
 
 
 def _rows_apart(name: str, t, row_stride: int) -> None:
@@ -91,14 +101,14 @@ def _device(**tensors) -> int:
     for name, t in tensors.items():
         if t is None:
             continue
-        if t.device.type != "cuda":
-            raise ValueError(f"{name} is on {t.device}, expected a CUDA device")
         if dev is None:
-            dev = t.device.index
-        elif t.device.index != dev:
-            raise ValueError(f"{name} is on {t.device}, the other tensors on cuda:{dev}")
-    runtime.init(dev)
-    return dev
+            dev = t.device
+            if dev.type != "cuda":
+                raise ValueError(f"{name} is on {dev}, expected a CUDA device")
+        elif t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {dev}")
+    runtime.init(dev.index)
+    return dev.index
 
 
 def _experts(n: int) -> None:
