@@ -377,7 +377,10 @@ int launch_variant(const Launch &l, bool tma, int pair, int bn) {
     if constexpr (LAYOUT == kMM) {
         return tma ? launch_single<I8, LAYOUT, 128, true>(l) : launch_single<I8, LAYOUT, 128, false>(l);
     } else {
-        if (!tma) return bn <= 32 ? launch_single<I8, LAYOUT, 32, false>(l) : launch_single<I8, LAYOUT, 128, false>(l);
+        if (!tma)
+            return bn == 32   ? launch_single<I8, LAYOUT, 32, false>(l)
+                   : bn == 64 ? launch_single<I8, LAYOUT, 64, false>(l)
+                              : launch_single<I8, LAYOUT, 128, false>(l);
         switch (bn) {
             case 16: return launch_single<I8, LAYOUT, 16, true>(l);
             case 32: return launch_single<I8, LAYOUT, 32, true>(l);
@@ -439,7 +442,17 @@ int launch_product(const Call &call, Product p, bool bf16) {
     // still fits; 64 until there are tiles for every SM (300 rows, [512, 1024]: 7.5 against 8.3 us at 128).
     int bn = 128;
     if (pair) bn = pair;
-    else if (!p.dw && !tma) bn = even <= 24 ? 32 : 128;
+    else if (!p.dw && !tma) {
+        // What a block costs the warps that cut it, relative to 128 wide: 0.63 and 0.48 (8787 rows, int8
+        // [639, 809]: 3 waves of tiles 128 wide in 68 us, 5 of 64 in 71, 10 of 32 in 108; 1022 rows, 8
+        // experts [777, 1001]: one wave of 128 in 50, one of 64 in 38, two of 32 in 52).
+        const struct { int bn; double cost; } widths[] = {{128, 1.0}, {64, 0.63}, {32, 0.48}};
+        double best = 1e300;
+        for (const auto &w : widths) {
+            const double cost = static_cast<double>(ceil_div(tiles(kTileM, w.bn), kSms)) * w.cost;
+            if (cost < best) best = cost, bn = w.bn;
+        }
+    }
     else if (!p.dw) bn = even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 || tiles(kTileM, 128) <= kSms ? 64 : 128;
 
     CUtensorMap ta{}, tb{};

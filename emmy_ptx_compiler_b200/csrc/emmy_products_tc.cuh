@@ -522,7 +522,7 @@ struct TcConfig {
     // two teams on alternate blocks hide more of the loads' latency (8 rows of 8 experts, int8 [3425,
     // 4057]: 94 against 125 us); with both operands 128 rows high they lack the registers (dw
     // [777, 1001] of 1022 rows: 54 against 38 us)
-    static constexpr int kTeams = BN == 32 ? 2 : 1;
+    static constexpr int kTeams = BN <= 64 ? 2 : 1;
     static constexpr int kLoaders = TMA ? 0 : 8 * kTeams;  // warps that load without TMA, 8 to a block
     static constexpr int kThreads = 64 + 32 * (kOut + kLoaders);
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + kOutStage + 256;

@@ -78,6 +78,9 @@ SHAPES = [
     ([300, 7, 300, 256, 0, 64, 257, 1000], 1536, 1032, 0),
     ([100, 64, 1, 128, 200, 0, 65, 130], 2604, 1544, 8),
     ([70, 1, 64, 0, 16, 63, 100, 17], 160, 2056, 0),
+    # odd rows, in tiles of 64 and of 128
+    ([221, 162, 129, 132, 103, 116, 84, 75], 777, 1001, 0),
+    ([128, 100, 156, 128, 0, 255, 128, 129], 2301, 135, 0),
     # enough tiles for a single CTA's widest
     ([60] * 8 + [50, 0, 61, 49, 50, 50, 64, 63], 2048, 2056, 0),
 ]
