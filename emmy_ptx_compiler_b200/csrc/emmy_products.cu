@@ -399,6 +399,71 @@ const void *end_of(const Operand &o, int esize) {
     return static_cast<const uint8_t *>(o.base) + last * esize;
 }
 
+// The kernel that a product runs on.
+struct Variant {
+    int pair = 0;      // 256 or 128: pairs of CTAs on tiles of as many output rows
+    int bn = 0;        // output rows of a tile
+    int split = 1;     // CTAs that divide a sum
+    int64_t clusters = 0;  // of the launch
+};
+
+// Chooses it by the extents, the operands' size and whether TMA can take both of them (`tma`); false where
+// the output has more tiles than are supported.
+bool choose(const Product &p, int esize, bool tma, Variant &v) {
+    // groups that can hold rows, and the rows of an even one
+    const int64_t groups = p.experts < p.rows ? p.experts : (p.rows ? p.rows : 1), bk = 128 / esize;
+    const int64_t even = ceil_div(p.rows, groups), kblocks = ceil_div(p.dw ? even : p.k, bk);
+    // tiles of even groups, and the most that any grouping can have
+    auto tiles = [&](int64_t tm, int64_t tc) {
+        return ceil_div(p.m, tm) * (p.dw ? p.experts * ceil_div(p.c, tc) : groups * ceil_div(even, tc));
+    };
+    auto most = [&](int64_t tm, int64_t tc) {
+        return ceil_div(p.m, tm) * (p.dw ? p.experts * ceil_div(p.c, tc) : p.rows / tc + groups);
+    };
+    if (most(kTileM, p.dw ? 64 : 16) > kMaxTiles) return false;
+    const int64_t cext = p.dw ? p.c : even;
+    // Pairs of CTAs where groups have rows for them and there are tiles enough, and, for dw, where the
+    // sums are long enough to cover a wide tile's way out (32 experts, dw [512, 1024]: 256 rows each 22
+    // against a single CTA's 19 us, 1000 rows each of 16 [1024, 1024] 36 against 47 us).
+    if (tma && p.m > 128 && cext > 64 && !(p.dw && kblocks < 8)) {
+        if (cext > 128 && tiles(256, 256) >= kSms / 4) v.pair = 256;
+        else if (tiles(256, 128) >= kSms / 4) v.pair = 128;
+    }
+    // Output rows of a single CTA's tile: a few more than an even group has, so that an uneven one
+    // still fits; 64 until there are tiles for every SM (300 rows, [512, 1024]: 7.5 against 8.3 us at 128).
+    v.bn = 128;
+    if (v.pair) v.bn = v.pair;
+    else if (!p.dw && !tma) {
+        // What a block costs the warps that cut it, relative to 128 wide: 0.63 and 0.48 (8787 rows, int8
+        // [639, 809]: 3 waves of tiles 128 wide in 68 us, 5 of 64 in 71, 10 of 32 in 108; 1022 rows, 8
+        // experts [777, 1001]: one wave of 128 in 50, one of 64 in 38, two of 32 in 52).
+        const struct { int bn; double cost; } widths[] = {{128, 1.0}, {64, 0.63}, {32, 0.48}};
+        double best = 1e300;
+        for (const auto &w : widths) {
+            const double cost = static_cast<double>(ceil_div(tiles(kTileM, w.bn), kSms)) * w.cost;
+            if (cost < best) best = cost, v.bn = w.bn;
+        }
+    }
+    else if (!p.dw) v.bn = even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 || tiles(kTileM, 128) <= kSms ? 64 : 128;
+    // CTAs that run at once: clusters of 4 and 8 leave some of a GPC's SMs over
+    auto resident = [&](int cluster) {
+        const int per_sm = !v.pair && tma && v.bn <= 32 ? 2 : 1;
+        return per_sm * (cluster <= 2 ? kSms : cluster == 4 ? 132 : 120);
+    };
+    // Idle SMs take parts of the sums, as long as a part is worth the exchange: 4 blocks of it for
+    // the few columns of a narrow tile, 8 (of 32 or more) and 16 for wider ones (1022 rows, 8 experts, dx
+    // [1000, 776], 13 blocks at 128 wide: 11 us whole, 18 in halves; 90 rows, [768, 8192]: 11 us in
+    // eighths, 13 in quarters; 60000 rows, dw [256, 256]: 275 us whole, 42 in eighths).
+    const int64_t part = v.bn <= 32 ? 4 : v.bn == 64 ? 8 : 16;
+    if (!v.pair && (v.bn != 64 || kblocks >= 32))
+        while (v.split < 8 && tiles(kTileM, v.bn) * v.split * 2 <= resident(v.split * 2) && kblocks >= v.split * 2 * part)
+            v.split *= 2;
+    const int cluster = v.pair ? 2 : v.split;
+    v.clusters = v.pair ? most(2 * kTileM, v.pair) : most(kTileM, v.bn);
+    if (v.clusters > resident(cluster) / cluster) v.clusters = resident(cluster) / cluster;
+    return true;
+}
+
 template <bool I8>
 int launch_product(const Call &call, Product p, bool bf16) {
     constexpr int esize = I8 ? 1 : 2, bk = 128 / esize;
@@ -416,80 +481,30 @@ int launch_product(const Call &call, Product p, bool bf16) {
     p.b_end = end_of(b, esize);
     const Flags flags{bf16, encode_tiled() && tma_ready(a, esize), encode_tiled() && tma_ready(b, esize)};
     const bool tma = flags.tma_a && flags.tma_b;
-
-    // groups that can hold rows, and the rows of an even one
-    const int64_t groups = p.experts < p.rows ? p.experts : (p.rows ? p.rows : 1);
-    const int64_t even = ceil_div(p.rows, groups), kblocks = ceil_div(p.dw ? even : p.k, bk);
-    // tiles of even groups, and the most that any grouping can have
-    auto tiles = [&](int64_t tm, int64_t tc) {
-        return ceil_div(p.m, tm) * (p.dw ? p.experts * ceil_div(p.c, tc) : groups * ceil_div(even, tc));
-    };
-    auto most = [&](int64_t tm, int64_t tc) {
-        return ceil_div(p.m, tm) * (p.dw ? p.experts * ceil_div(p.c, tc) : p.rows / tc + groups);
-    };
-    const int64_t cext = p.dw ? p.c : even;
-    // Pairs of CTAs where groups have rows for them and there are tiles enough, and, for dw, where the
-    // sums are long enough to cover a wide tile's way out (32 experts, dw [512, 1024]: 256 rows each 22
-    // against a single CTA's 19 us, 1000 rows each of 16 [1024, 1024] 36 against 47 us).
-    int pair = 0;
-    if (tma && p.m > 128 && cext > 64 && !(p.dw && kblocks < 8)) {
-        if (cext > 128 && tiles(256, 256) >= kSms / 4) pair = 256;
-        else if (tiles(256, 128) >= kSms / 4) pair = 128;
-    }
-    if (most(kTileM, p.dw ? 64 : 16) > kMaxTiles)
+    Variant v;
+    if (!choose(p, esize, tma, v))
         return report(EMMY_ERR_INVALID, "%s: an output of more than 2^30 tiles is not supported", call.name);
-    // Output rows of a single CTA's tile: a few more than an even group has, so that an uneven one
-    // still fits; 64 until there are tiles for every SM (300 rows, [512, 1024]: 7.5 against 8.3 us at 128).
-    int bn = 128;
-    if (pair) bn = pair;
-    else if (!p.dw && !tma) {
-        // What a block costs the warps that cut it, relative to 128 wide: 0.63 and 0.48 (8787 rows, int8
-        // [639, 809]: 3 waves of tiles 128 wide in 68 us, 5 of 64 in 71, 10 of 32 in 108; 1022 rows, 8
-        // experts [777, 1001]: one wave of 128 in 50, one of 64 in 38, two of 32 in 52).
-        const struct { int bn; double cost; } widths[] = {{128, 1.0}, {64, 0.63}, {32, 0.48}};
-        double best = 1e300;
-        for (const auto &w : widths) {
-            const double cost = static_cast<double>(ceil_div(tiles(kTileM, w.bn), kSms)) * w.cost;
-            if (cost < best) best = cost, bn = w.bn;
-        }
-    }
-    else if (!p.dw) bn = even <= 12 ? 16 : even <= 24 ? 32 : even <= 48 || tiles(kTileM, 128) <= kSms ? 64 : 128;
-
     CUtensorMap ta{}, tb{};
     const CUtensorMapDataType type = I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                      : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if ((flags.tma_a && !encode(&ta, a, type, esize, 3, bk, a_mn ? 64 : kTileM)) ||
-        (flags.tma_b && !encode(&tb, b, type, esize, 2, bk, p.dw ? 64 : pair ? pair / 2 : bn)))
+        (flags.tma_b && !encode(&tb, b, type, esize, 2, bk, p.dw ? 64 : v.pair ? v.pair / 2 : v.bn)))
         return report(EMMY_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", call.name);
-    // CTAs that run at once: clusters of 4 and 8 leave some of a GPC's SMs over
-    auto resident = [&](int cluster) {
-        const int per_sm = !pair && tma && bn <= 32 ? 2 : 1;
-        return per_sm * (cluster <= 2 ? kSms : cluster == 4 ? 132 : 120);
-    };
-    // Idle SMs take parts of the sums, as long as a part is worth the exchange: 4 blocks of it for
-    // the few columns of a narrow tile, 8 (of 32 or more) and 16 for wider ones (1022 rows, 8 experts, dx
-    // [1000, 776], 13 blocks at 128 wide: 11 us whole, 18 in halves; 90 rows, [768, 8192]: 11 us in
-    // eighths, 13 in quarters; 60000 rows, dw [256, 256]: 275 us whole, 42 in eighths).
-    const int64_t part = bn <= 32 ? 4 : bn == 64 ? 8 : 16;
-    int split = 1;
-    if (!pair && (bn != 64 || kblocks >= 32))
-        while (split < 8 && tiles(kTileM, bn) * split * 2 <= resident(split * 2) && kblocks >= split * 2 * part) split *= 2;
-    const int cluster = pair ? 2 : split;
-    int64_t clusters = pair ? most(2 * kTileM, pair) : most(kTileM, bn);
-    if (clusters > resident(cluster) / cluster) clusters = resident(cluster) / cluster;
-    const Launch l{call, p, flags, ta, tb, clusters, cluster};
+    const Launch l{call, p, flags, ta, tb, v.clusters, v.pair ? 2 : v.split};
     if constexpr (I8) {
-        return launch_variant<true, kKK>(l, tma, pair, bn);
+        return launch_variant<true, kKK>(l, tma, v.pair, v.bn);
     } else {
-        return p.dw ? launch_variant<false, kMM>(l, tma, pair, bn)
-               : a_mn ? launch_variant<false, kMK>(l, tma, pair, bn)
-                      : launch_variant<false, kKK>(l, tma, pair, bn);
+        return p.dw ? launch_variant<false, kMM>(l, tma, v.pair, v.bn)
+               : a_mn ? launch_variant<false, kMK>(l, tma, v.pair, v.bn)
+                      : launch_variant<false, kKK>(l, tma, v.pair, v.bn);
     }
 }
 
+bool no_output(const Product &p) { return p.m == 0 || p.experts == 0 || (p.dw ? p.c : p.rows) == 0; }
+
 int run_product(const char *name, int dev, int operands, const Product &p, uint64_t stream) {
-    if (p.m == 0 || p.experts == 0 || (p.dw ? p.c : p.rows) == 0) return EMMY_OK;
+    if (no_output(p)) return EMMY_OK;
     DeviceScope scope(dev);
     if (scope.err != cudaSuccess)
         return report(EMMY_ERR_CUDA, "%s: device %d: %s", name, dev, cudaGetErrorString(scope.err));
@@ -629,6 +644,24 @@ extern "C" int emmy_quantize_rows(int dev, int dtype, const void *x, int64_t x_s
     if (dtype == EMMY_BF16) return launch_quantize(call, static_cast<const __nv_bfloat16 *>(x), x_stride, q, q_stride, scale, rows, k);
     if (dtype == EMMY_F16) return launch_quantize(call, static_cast<const __half *>(x), x_stride, q, q_stride, scale, rows, k);
     return launch_quantize(call, static_cast<const float *>(x), x_stride, q, q_stride, scale, rows, k);
+}
+
+extern "C" int emmy_products_variant(int esize, int dw, int aligned, int64_t rows, int64_t experts, int64_t n,
+                                     int64_t k, int32_t *variant) {
+    static const char name[] = "emmy_products_variant";
+    if (int rc = check_common(name, 0, rows, experts, n, k)) return rc;
+    if ((esize != 1 && esize != 2) || (dw && esize == 1))
+        return report(EMMY_ERR_INVALID, "%s: operands of 2 bytes, or of 1 where dw is 0", name);
+    if (!variant) return report(EMMY_ERR_INVALID, "%s: NULL pointer", name);
+    Product p{};
+    p.m = dw ? k : n, p.c = dw ? n : 0, p.k = dw ? 0 : k, p.rows = rows;
+    p.experts = static_cast<int>(experts), p.dw = dw != 0;
+    Variant v;
+    // without rows or terms of a sum there is nothing for TMA to load
+    if (!no_output(p) && !choose(p, esize, aligned && rows && k, v))
+        return report(EMMY_ERR_INVALID, "%s: an output of more than 2^30 tiles is not supported", name);
+    variant[0] = v.pair != 0, variant[1] = v.bn, variant[2] = v.split;
+    return EMMY_OK;
 }
 
 extern "C" int emmy_products_status(int dev, uint32_t *status) {

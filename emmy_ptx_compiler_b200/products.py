@@ -247,6 +247,18 @@ def quantize_rows(x, q, scale, stream: int = 0) -> None:
     bind_quantize_rows(x, q, scale, stream)()
 
 
+def variant(rows: int, experts: int, n: int, k: int, dw: bool = False, esize: int = 2,
+            aligned: bool = True) -> tuple[bool, int, int]:
+    """The kernel that a product of these extents runs on: whether pairs of CTAs, the output rows of a
+    tile (0: nothing to launch), and how many CTAs divide a sum.
+
+    ``dw`` asks for :func:`grouped_matmul_dw`, ``esize`` 1 for :func:`int8_matmul`; ``aligned`` says that
+    both operands' bases and strides are multiples of 16 bytes.  Needs no GPU."""
+    v = (C.c_int32 * 3)()
+    runtime._check(runtime.lib().emmy_products_variant(esize, dw, aligned, rows, experts, n, k, v))
+    return bool(v[0]), v[1], v[2]
+
+
 def status(device: int = 0) -> int:
     """Read and clear the EMMY_STATUS_* bits of these kernels on ``device`` (0: every wait ended in
     time); synchronises the device."""

@@ -64,6 +64,7 @@ def _declare(lib) -> None:
         "emmy_grouped_matmul_dw": ([i32, i32, i32, vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, i64, i64, u64], i32),
         "emmy_int8_matmul": ([i32, i32, vp, i64, vp, vp, i64, i64, vp, vp, vp, vp, i64, i64, i64, i64, i64, u64], i32),
         "emmy_quantize_rows": ([i32, i32, vp, i64, vp, i64, vp, i64, i64, u64], i32),
+        "emmy_products_variant": ([i32, i32, i32, i64, i64, i64, i64, P(C.c_int32)], i32),
         "emmy_products_status": ([i32, P(u32)], i32),
         "emmy_xchg_create": ([i32, i32, i32, P(vp), P(C.c_uint8)], i32),
         "emmy_xchg_connect": ([vp, P(C.c_uint8)], i32),
@@ -95,7 +96,7 @@ EXPORTED = ("emmy_version", "emmy_last_error", "emmy_init", "emmy_device_count",
             "emmy_host_alloc", "emmy_host_free", "emmy_run_host", "emmy_time_launch", "emmy_launch_range",
             "emmy_module_range", "emmy_shard_range", "emmy_launch_sharded", "emmy_sum_f32_noalloc",
             "emmy_grouped_matmul", "emmy_grouped_matmul_dw", "emmy_int8_matmul", "emmy_quantize_rows",
-            "emmy_products_status",
+            "emmy_products_variant", "emmy_products_status",
             "emmy_xchg_create", "emmy_xchg_connect", "emmy_sum_f32_allreduce", "emmy_xchg_status",
             "emmy_xchg_reset", "emmy_launch_xchg", "emmy_xchg_destroy",
             "emmy_comm_unique_id", "emmy_comm_init", "emmy_allreduce_f32", "emmy_allgather_f32",

@@ -231,6 +231,13 @@ int emmy_sum_f32_noalloc(int dev, const float *x, uint64_t n, float *out, uint64
  *                           ties to even), within [-127, 127].  A row of zeros
  *                           gives scale 0 and zeros; a row that holds an
  *                           infinity or NaN gives scale NaN and zeros.
+ *   emmy_products_variant   the kernel that a product of these extents runs on:
+ *                           variant[0] is 1 for pairs of CTAs, variant[1] the output
+ *                           rows of a tile (0: nothing to launch), variant[2] the CTAs
+ *                           that divide a sum.  `esize` is the operands' size (1 or 2),
+ *                           `dw` 1 for emmy_grouped_matmul_dw, `aligned` 1 where both
+ *                           operands' bases and strides are multiples of 16 bytes.
+ *                           Needs no GPU.
  *   emmy_products_status    reads and clears the device's EMMY_STATUS_* bits of
  *                           these kernels (a bounded wait that ran out, whose
  *                           outputs are then undefined); synchronises the device. */
@@ -251,6 +258,8 @@ int emmy_int8_matmul(int dev, int out_dtype, const int8_t *xq, int64_t x_stride,
                      int64_t experts, int64_t n, int64_t k, uint64_t stream);
 int emmy_quantize_rows(int dev, int dtype, const void *x, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
                        int64_t rows, int64_t k, uint64_t stream);
+int emmy_products_variant(int esize, int dw, int aligned, int64_t rows, int64_t experts, int64_t n, int64_t k,
+                          int32_t variant[3]);
 int emmy_products_status(int dev, uint32_t *status);
 
 /* The C4 step on N GPUs as ONE kernel per GPU (no counterpart in the

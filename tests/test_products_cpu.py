@@ -140,3 +140,45 @@ def test_calls_without_work_need_no_gpu():
     assert lib.emmy_grouped_matmul_dw(*{**DW, "experts": 0}.values()) == 0
     assert lib.emmy_quantize_rows(*{**QUANTIZE, "rows": 0}.values()) == 0
     assert lib.emmy_products_status(0, None) == -3
+
+
+def test_the_kernel_that_a_product_runs_on():
+    assert products.variant(0, 3, 64, 64) == (False, 0, 1)            # nothing to launch
+    assert products.variant(0, 3, 64, 64, dw=True) == (False, 128, 1)  # zeros to write
+    assert products.variant(5, 1, 64, 0) == products.variant(5, 1, 64, 0, aligned=False)
+    for bad in (dict(rows=-1), dict(experts=1025), dict(esize=3), dict(esize=1, dw=True),
+                dict(rows=1 << 30, n=1 << 30)):
+        with pytest.raises(runtime.EmmyError):
+            products.variant(**{**dict(rows=5, experts=2, n=64, k=64), **bad})
+
+
+def test_the_gpu_tests_reach_every_kernel():
+    """A change of the rule that picks kernels must not take one away from the cases that test it."""
+    import test_products_gpu as gpu
+
+    forward, rows_gradient, int8, dw = set(), set(), set(), set()
+
+    def aligned(unit, *strides):
+        return all(s % unit == 0 for s in strides)
+
+    for counts, n, k, pad in gpu.SHAPES:
+        rows, e = sum(counts), len(counts)
+        a = aligned(8, k + pad)
+        forward.add((a, products.variant(rows + 5, e, n, k, aligned=a)[:2]))
+        a = aligned(8, k + pad, n + pad)
+        rows_gradient.add((a, products.variant(rows, e, k, n, aligned=a)[:2]))
+        dw.add((a, products.variant(rows + 8, e, n, k, dw=True, aligned=a)[:2]))
+    for counts, grouped, n, k, pad in gpu.INT8_SHAPES:
+        a = aligned(16, k + pad)
+        int8.add((a, products.variant(sum(counts) + (4 if grouped else 0), len(counts), n, k, esize=1, aligned=a)[:2]))
+    for counts, n, k, esize, kernel in gpu.WIDTHS:
+        a = aligned(16 // esize, k)
+        for s in (int8,) if esize == 1 else (forward, rows_gradient):
+            s.add((a, kernel[:2]))
+    rows = sum(gpu.PAIR_COUNTS) + 8
+    for n, k, width in gpu.DW_PAIRS:
+        dw.add((True, products.variant(rows, len(gpu.PAIR_COUNTS), n, k, dw=True)[:2]))
+    every = {(True, (False, w)) for w in (16, 32, 64, 128)} | {(False, (False, w)) for w in (32, 64, 128)}
+    every |= {(True, (True, w)) for w in (128, 256)}
+    assert forward == every and rows_gradient == every and int8 == every
+    assert dw == {(True, (False, 128)), (False, (False, 128)), (True, (True, 128)), (True, (True, 256))}

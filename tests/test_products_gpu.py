@@ -716,3 +716,144 @@ def test_two_host_threads_at_once():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not errors and torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def _ints(g, *shape, dtype=BF16, pad=0):
+    """Values whose sums of up to 2^24 / 9 products are exact in f32, in rows ``pad`` apart."""
+    return torch.randint(-3, 4, (*shape[:-1], shape[-1] + pad), device="cuda", generator=g).to(dtype)[..., :shape[-1]]
+
+
+# rows of each expert of gradients that run on pairs of CTAs: last blocks of 1, 15, 16, 17, 63, 64 rows, an
+# empty group, groups that end on a block between others, a single row
+PAIR_COUNTS = [513, 527, 528, 529, 575, 512, 576, 0, 1, 64, 1100, 640]
+# n, k, rows of a tile; the first has several tiles for each pair of CTAs
+DW_PAIRS = [(1032, 1032, 256), (264, 384, 256), (104, 776, 128), (200, 392, 128)]
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(BF16, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("n,k,width", DW_PAIRS)
+def test_dw_on_pairs_of_ctas(n, k, width, dtype, out_dtype):
+    """Against exact sums, in two orders of the groups, with infinities and NaN in some groups and
+    outside all of them."""
+    g = _gen(n + k)
+    first, spare, pad = 3, 5, 8
+    rows, e = first + sum(PAIR_COUNTS) + spare, len(PAIR_COUNTS)
+    assert products.variant(rows, e, n, k, dw=True) == (True, width, 1)
+    dw = torch.full((e, n, k + pad), 7.0, dtype=out_dtype, device="cuda")[..., :k]
+    for counts in (PAIR_COUNTS, PAIR_COUNTS[::-1]):
+        dy, x = _ints(g, rows, n, dtype=dtype, pad=pad), _ints(g, rows, k, dtype=dtype)
+        off = _offsets(counts, first)
+        ends = off.tolist()
+        lost = [counts.index(528), counts.index(64)]
+        for a, b in [(0, first), (rows - spare, rows)] + [(ends[i], ends[i + 1]) for i in lost]:
+            dy[a:b], x[a:b] = float("inf"), float("nan")
+        for _ in range(3):
+            products.grouped_matmul_dw(dy, x, off, dw, stream=_stream())
+        for i in range(e):
+            r = slice(ends[i], ends[i + 1])
+            if i in lost:
+                assert dw[i].isnan().all()
+            else:
+                want = (dy[r].double().t() @ x[r].double()).float().to(out_dtype)
+                assert torch.equal(dw[i], want), (i, counts[i])
+        assert (dw.as_strided((e, n, pad), dw.stride(), dw.storage_offset() + k) == 7).all()
+
+
+def test_dw_on_pairs_of_ctas_recorded():
+    """A recorded call follows new offsets, whichever of the groups end inside a block."""
+    g = _gen(41)
+    n, k, e = 264, 384, len(PAIR_COUNTS)
+    rows = sum(PAIR_COUNTS)
+    assert products.variant(rows, e, n, k, dw=True)[0]
+    dy, x, off = _ints(g, rows, n), _ints(g, rows, k), _offsets(PAIR_COUNTS)
+    dw = torch.empty(e, n, k, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with runtime.Graph.record(0, s.cuda_stream) as graph:
+        products.grouped_matmul_dw(dy, x, off, dw, stream=s.cuda_stream)
+    for counts in (PAIR_COUNTS, sorted(PAIR_COUNTS), [0] * (e - 1) + [rows], [rows - 11] + [1] * (e - 1), [64] * e):
+        off.copy_(_offsets(counts))
+        dw.fill_(7)
+        torch.cuda.synchronize()
+        graph.launch(s.cuda_stream)
+        torch.cuda.synchronize()
+        at = 0
+        for i, c in enumerate(counts):
+            assert torch.equal(dw[i].double(), dy[at:at + c].double().t() @ x[at:at + c].double()), (counts, i)
+            at += c
+    graph.close()
+
+
+# rows of each expert, n, k, operands' size, the kernel: tiles that the shapes above do not reach
+WIDTHS = [
+    ([20, 14, 24], 136, 136, 2, (False, 32, 1)),
+    ([1700], 1100, 65, 2, (False, 128, 1)),
+    ([700], 1100, 65, 1, (False, 64, 1)),
+    ([1700], 1100, 65, 1, (False, 128, 1)),
+    ([60] * 16, 1300, 144, 1, (False, 128, 1)),
+]
+# sums divided among 2, 4 and 8 CTAs, for each width of a tile
+SPLITS = [
+    ([40], 2080, 1025, 2, (False, 32, 2)),
+    ([9], 136, 1025, 2, (False, 32, 4)),
+    ([9], 136, 4097, 2, (False, 32, 8)),
+    ([9], 136, 1024, 2, (False, 16, 4)),
+    ([9], 136, 4096, 2, (False, 16, 8)),
+    ([20], 136, 1024, 2, (False, 32, 4)),
+    ([20], 136, 4096, 2, (False, 32, 8)),
+    ([100], 2080, 4096, 2, (False, 64, 2)),
+    ([40], 2080, 4096, 2, (False, 64, 4)),
+    ([40], 136, 4096, 2, (False, 64, 8)),
+    ([9], 136, 1024, 1, (False, 16, 2)),
+    ([9], 4112, 4096, 1, (False, 16, 4)),
+    ([9], 136, 4096, 1, (False, 16, 8)),
+    ([20], 136, 1024, 1, (False, 32, 2)),
+    ([20], 4112, 4096, 1, (False, 32, 4)),
+    ([20], 136, 4096, 1, (False, 32, 8)),
+    ([100], 2080, 4096, 1, (False, 64, 2)),
+    ([40], 136, 4096, 1, (False, 64, 4)),
+    ([40], 136, 8192, 1, (False, 64, 8)),
+    ([9], 136, 1025, 1, (False, 32, 2)),
+    ([9], 2080, 4097, 1, (False, 32, 4)),
+    ([9], 136, 4097, 1, (False, 32, 8)),
+]
+
+
+@pytest.mark.parametrize("counts,n,k,esize,kernel", WIDTHS + SPLITS)
+def test_tile_widths_and_split_sums(counts, n, k, esize, kernel):
+    g = _gen(n + k + esize)
+    rows, e = sum(counts), len(counts)
+    assert products.variant(rows, e, n, k, esize=esize, aligned=k % (16 // esize) == 0) == kernel
+    off, out = _offsets(counts), torch.empty(rows, n, device="cuda")
+    x, w = _ints(g, rows, k), _ints(g, e, n, k)
+    if esize == 1:
+        one = torch.ones(e, max(n, rows), device="cuda")
+        products.int8_matmul(x.to(torch.int8), one[0, :rows], w.to(torch.int8), one[:, :n].contiguous(), out, offsets=off,
+                             stream=_stream())
+    else:
+        products.grouped_matmul(x, w, off, out, stream=_stream())
+        # weights whose n axis is contiguous take the same kernels' other layout
+        wt = _ints(g, e, k, n).transpose(1, 2)
+        out2 = torch.empty_like(out)
+        products.grouped_matmul(x, wt, off, out2, stream=_stream())
+    at = 0
+    for i, c in enumerate(counts):
+        X = x[at:at + c].double()
+        assert torch.equal(out[at:at + c].double(), X @ w[i].double().t())
+        if esize == 2:
+            assert torch.equal(out2[at:at + c].double(), X @ wt[i].double().t())
+        at += c
+
+
+@pytest.mark.parametrize("rows,n,k,split", [(2100, 72, 72, 2), (4100, 72, 72, 4), (9000, 72, 72, 8), (2100, 72, 71, 2),
+                                            (4100, 71, 72, 4), (9001, 71, 71, 8), (20011, 264, 200, 8)])
+def test_split_sums_of_dw_are_exact(rows, n, k, split):
+    """Every row counts once: integers whose sums of any order are exact, some rows outside the group."""
+    g = _gen(rows + n)
+    aligned = n % 8 == 0 and k % 8 == 0
+    assert products.variant(rows + 7, 1, n, k, dw=True, aligned=aligned) == (False, 128, split)
+    dy, x = _ints(g, rows + 7, n), _ints(g, rows + 7, k)
+    dy[:2], x[:2], dy[-5:], x[-5:] = float("nan"), float("inf"), float("inf"), float("nan")
+    dw = torch.full((1, n, k), 7.0, device="cuda")
+    products.grouped_matmul_dw(dy, x, torch.tensor([2, rows + 2], dtype=torch.int32, device="cuda"), dw, stream=_stream())
+    assert torch.equal(dw[0].double(), dy[2:-5].double().t() @ x[2:-5].double())
