@@ -142,9 +142,9 @@ __host__ __device__ constexpr uint32_t idesc_s8(uint32_t m, uint32_t n) {
 
 namespace {
 
-constexpr uint64_t kWaitNs = 2000000000ull;  // per wait: orders of magnitude above any legal one
-// A wait for a whole sum may last as long as its blocks do, at 20 us each (0.3 to 2 us measured).
-__device__ __forceinline__ uint64_t sum_wait_ns(int blocks) { return kWaitNs + static_cast<uint64_t>(blocks) * 20000ull; }
+constexpr uint64_t kWaitNs = 2000000000ull;  // a wait for one block or one tile's way out: orders of magnitude above any legal one
+// A wait for whole sums may last as long as their blocks do, at 20 us each (0.3 to 2 us measured).
+__device__ __forceinline__ uint64_t sum_wait_ns(uint64_t blocks) { return kWaitNs + blocks * 20000ull; }
 constexpr int kTileM = 128;
 constexpr uint32_t kBlockBytes = 128;                  // one 128-byte swizzle row of k (or of m, c)
 constexpr uint32_t kPanel = 64 * kBlockBytes;          // 64 k x 64 m (or c) of an MN-major 16-bit operand
@@ -1097,15 +1097,18 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
         // next group, or hold anything.  What the last MMA takes of them becomes zero in both
         // operands before the leader's barrier completes, while the loads run on.
         uint32_t blocks = 0, tail_parity = 0u;  // of `tail`, one bit for each stage
+        uint64_t span = 0;  // what a wait lasts: every sum since the last tile that ended inside, and its way out
         for (int t = pair; t < total; t += npairs) {
             const Tile w = tile(t);
             blocks += w.kb1;
+            span += w.kb1 + 1;
             const int have = w.kend % BK;
             if (have == 0) continue;
             const uint32_t stage = (blocks - 1) % STAGES;
             if (!__all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tail[stage], tail_parity >> stage & 1u, abort_flag,
-                                                                 EMMY_STATUS_TIMEOUT_PRODUCER, kWaitNs)))
+                                                                 EMMY_STATUS_TIMEOUT_PRODUCER, sum_wait_ns(span))))
                 break;
+            span = 0;
             tail_parity ^= 1u << stage;
             const int upto = (have + 15) / 16 * 16;
             for (int j = 0; j < 2; ++j) zero_panel_rows(sA + stage * kStageA + j * kPanel, have, upto, lane);

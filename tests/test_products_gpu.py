@@ -857,3 +857,24 @@ def test_split_sums_of_dw_are_exact(rows, n, k, split):
     dw = torch.full((1, n, k), 7.0, device="cuda")
     products.grouped_matmul_dw(dy, x, torch.tensor([2, rows + 2], dtype=torch.int32, device="cuda"), dw, stream=_stream())
     assert torch.equal(dw[0].double(), dy[2:-5].double().t() @ x[2:-5].double())
+
+
+def test_a_launch_of_more_than_two_seconds():
+    """The blocks that end inside come last, in an expert of their own: what waits for them waits for
+    the whole launch, 4e15 operations (2.4 s at 1.65 PFLOP/s), and this is no failure."""
+    n, rows, last = 73728, 368_000, 33
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 85 << 30:
+        pytest.skip("needs 76 GB of device memory")
+    assert rows % 64 == 0 and products.variant(rows + last, 2, n, n, dw=True) == (True, 256, 1)
+    x = torch.empty(rows + last, n, dtype=BF16, device="cuda").random_(-3, 4, generator=_gen(51))
+    dw = torch.empty(2, n, n, dtype=BF16, device="cuda")
+    products.grouped_matmul_dw(x, x, _offsets([rows, last]), dw, stream=_stream())
+    torch.cuda.synchronize()
+    assert products.status(0) == 0
+    for i, r in enumerate((slice(0, rows), slice(rows, rows + last))):
+        for a, b in ((0, 0), (n - 64, 256), (4096, n - 64)):
+            want = x[r, a:a + 64].double().t() @ x[r, b:b + 64].double()   # exact in f32, rounded once
+            assert torch.equal(dw[i, a:a + 64, b:b + 64], want.float().to(BF16)), (i, a, b)
+    del x, dw
+    torch.cuda.empty_cache()
