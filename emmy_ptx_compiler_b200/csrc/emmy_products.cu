@@ -14,9 +14,8 @@
 //
 // The group boundaries are read on the device; a launch covers any of them, so no call waits for
 // the host and a recorded graph follows new boundaries.  Sums of 16-bit products are held in f32 and
-// rounded once, to the output's type; tensor cores truncate where they align addends, so a sum of k
-// terms is off by up to k steps of 2^-23 of its magnitude rather than half steps.  Sums of 8-bit
-// products are exact in s32; scaling rounds them to f32 (a 24-bit significand, for sums beyond 2^24),
+// rounded once, to the output's type; tensor cores truncate where they align addends, so long sums are
+// joined from segments.  Sums of 8-bit products are exact in s32; scaling rounds them to f32 (a 24-bit significand, for sums beyond 2^24),
 // then once for each scale, the bias and the output's type.
 
 #include <cuda.h>
@@ -356,36 +355,36 @@ int launch_clusters(const Launch &l, TcKernel kernel, std::atomic<uint64_t> &rea
     return launched(l.call, cudaLaunchKernelEx(&cfg, kernel, l.p, l.flags, l.ta, l.tb));
 }
 
-template <bool I8, int LAYOUT, int BN, bool TMA>
+template <bool I8, int LAYOUT, int BN, bool TMA, bool JOIN>
 int launch_single(const Launch &l) {
     using Cfg = TcConfig<I8, BN, TMA>;
     static std::atomic<uint64_t> ready{0};
-    return launch_clusters(l, product_tc_kernel<I8, LAYOUT, BN, TMA>, ready, Cfg::kThreads, Cfg::kSmem);
+    return launch_clusters(l, product_tc_kernel<I8, LAYOUT, BN, TMA, JOIN>, ready, Cfg::kThreads, Cfg::kSmem);
 }
 
-template <bool I8, int LAYOUT, int BN>
+template <bool I8, int LAYOUT, int BN, bool JOIN>
 int launch_pair(const Launch &l) {
     using Cfg = PairConfig<BN>;
     static std::atomic<uint64_t> ready{0};
-    return launch_clusters(l, product_pair_kernel<I8, LAYOUT, BN>, ready,
+    return launch_clusters(l, product_pair_kernel<I8, LAYOUT, BN, JOIN>, ready,
                            Cfg::kThreads + (LAYOUT == kMM ? Cfg::kTailThreads : 0), Cfg::kSmem);
 }
 
-template <bool I8, int LAYOUT>
+template <bool I8, int LAYOUT, bool JOIN>
 int launch_variant(const Launch &l, bool tma, int pair, int bn) {
-    if (pair) return pair == 256 ? launch_pair<I8, LAYOUT, 256>(l) : launch_pair<I8, LAYOUT, 128>(l);
+    if (pair) return pair == 256 ? launch_pair<I8, LAYOUT, 256, JOIN>(l) : launch_pair<I8, LAYOUT, 128, JOIN>(l);
     if constexpr (LAYOUT == kMM) {
-        return tma ? launch_single<I8, LAYOUT, 128, true>(l) : launch_single<I8, LAYOUT, 128, false>(l);
+        return tma ? launch_single<I8, LAYOUT, 128, true, JOIN>(l) : launch_single<I8, LAYOUT, 128, false, JOIN>(l);
     } else {
         if (!tma)
-            return bn == 32   ? launch_single<I8, LAYOUT, 32, false>(l)
-                   : bn == 64 ? launch_single<I8, LAYOUT, 64, false>(l)
-                              : launch_single<I8, LAYOUT, 128, false>(l);
+            return bn == 32   ? launch_single<I8, LAYOUT, 32, false, JOIN>(l)
+                   : bn == 64 ? launch_single<I8, LAYOUT, 64, false, JOIN>(l)
+                              : launch_single<I8, LAYOUT, 128, false, JOIN>(l);
         switch (bn) {
-            case 16: return launch_single<I8, LAYOUT, 16, true>(l);
-            case 32: return launch_single<I8, LAYOUT, 32, true>(l);
-            case 64: return launch_single<I8, LAYOUT, 64, true>(l);
-            default: return launch_single<I8, LAYOUT, 128, true>(l);
+            case 16: return launch_single<I8, LAYOUT, 16, true, JOIN>(l);
+            case 32: return launch_single<I8, LAYOUT, 32, true, JOIN>(l);
+            case 64: return launch_single<I8, LAYOUT, 64, true, JOIN>(l);
+            default: return launch_single<I8, LAYOUT, 128, true, JOIN>(l);
         }
     }
 }
@@ -493,11 +492,17 @@ int launch_product(const Call &call, Product p, bool bf16) {
         return report(EMMY_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", call.name);
     const Launch l{call, p, flags, ta, tb, v.clusters, v.pair ? 2 : v.split};
     if constexpr (I8) {
-        return launch_variant<true, kKK>(l, tma, v.pair, v.bn);
+        return launch_variant<true, kKK, false>(l, tma, v.pair, v.bn);
     } else {
-        return p.dw ? launch_variant<false, kMM>(l, tma, v.pair, v.bn)
-               : a_mn ? launch_variant<false, kMK>(l, tma, v.pair, v.bn)
-                      : launch_variant<false, kKK>(l, tma, v.pair, v.bn);
+        // the longest sum that a CTA may have
+        const bool join = ceil_div(ceil_div(p.dw ? p.rows : p.k, bk), v.split) > segment_blocks(p.out_type);
+        auto go = [&](auto kernels) {
+            constexpr bool JOIN = decltype(kernels)::value;
+            return p.dw ? launch_variant<false, kMM, JOIN>(l, tma, v.pair, v.bn)
+                   : a_mn ? launch_variant<false, kMK, JOIN>(l, tma, v.pair, v.bn)
+                          : launch_variant<false, kKK, JOIN>(l, tma, v.pair, v.bn);
+        };
+        return join ? go(std::true_type{}) : go(std::false_type{});
     }
 }
 

@@ -495,6 +495,116 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
     }
 }
 
+// Tensor cores cut off what lies below the last bit of a running sum, so a long sum of one sign would
+// lose up to half a step for each MMA (262144 rows of positive values: 1.5e-3 of their sum).  So sums of
+// 16-bit products are joined from segments, added in f32 to nearest by the warps that turn sums into
+// output: 1024 terms for an f32 output (1e-6 off for values of either sign, 1.7e-6 for values of one), 8192
+// where rounding to 16 bits follows (3e-5 of a sum of one sign; half a step is 4.9e-4 or 3.9e-3).
+// Kernels with JOIN do so, at 0 to 4 % more time (4 experts of 16384 rows, dw [2048, 2048]: 391 against
+// 385 us to bf16, 398 against 388 to f32); where no sum of a launch can be that long the others run.
+constexpr int kShortSegment = 16, kLongSegment = 128;  // blocks
+__host__ __device__ constexpr int segment_blocks(int out_type) { return out_type == EMMY_F32 ? kShortSegment : kLongSegment; }
+// Segments of a sum after the first.
+__device__ __forceinline__ int more_segments(int blocks, int segment) { return blocks > segment ? (blocks - 1) / segment : 0; }
+
+// The barriers of a tile's accumulators: segment `it` of a CTA's tiles arrives in accumulator `it` & 1.
+template <bool PAIR>
+struct Accumulators {
+    uint64_t *full, *empty;  // it is complete; it may be overwritten (PAIR: the leader's counts)
+    volatile uint32_t *abort_flag;
+
+    __device__ __forceinline__ bool wait(uint32_t it, int blocks) const {
+        uint64_t *bar = &full[it & 1u];
+        const uint32_t phase = (it >> 1) & 1u;
+        const bool ok = PAIR ? emmy::mbar_wait_cluster(bar, phase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, sum_wait_ns(blocks))
+                             : emmy::mbar_wait(bar, phase, abort_flag, EMMY_STATUS_TIMEOUT_EPILOGUE, sum_wait_ns(blocks));
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        emmy::tc_fence_after();
+        return true;
+    }
+    __device__ __forceinline__ void release(uint32_t it, int lane) const {
+        emmy::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            if constexpr (PAIR) emmy::mbar_arrive_cluster(emmy::mapa(&empty[it & 1u], 0));
+            else emmy::mbar_arrive(&empty[it & 1u]);
+        }
+    }
+};
+
+// The sum of the segments `it` to `it` + `more` of a tile, for a warp's 32 channels and the SPAN columns
+// from `taddr` of the first accumulator on (the second one is BN columns further), left in the columns behind
+// both.  Every accumulator is released.
+template <int BN, int SPAN, bool PAIR>
+__device__ __forceinline__ bool join_segments(uint32_t taddr, const Accumulators<PAIR> acc, uint32_t it, int more, int lane) {
+    const uint32_t whole = taddr + 2 * BN;
+    #pragma unroll 1
+    for (int s = 0; s <= more; ++s, ++it) {
+        if (!acc.wait(it, kLongSegment)) return false;
+        #pragma unroll 1
+        for (int c = 0; c < SPAN; c += 16) {
+            uint32_t r[16], sum[16];
+            emmy::tmem_ld_32x32b_x16(taddr + (it & 1u) * BN + c, r);
+            if (s > 0) emmy::tmem_ld_32x32b_x16(whole + c, sum);
+            emmy::tmem_ld_wait();
+            #pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (s > 0) r[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(r[j]));
+            emmy::tmem_st_32x32b_x16(whole + c, r);
+        }
+        emmy::tmem_st_wait();
+        acc.release(it, lane);
+    }
+    return true;
+}
+
+// Out of line, for kernels whose warps that load leave few registers.
+template <int BN, int SPAN, bool PAIR>
+__device__ __noinline__ bool join_segments_apart(uint32_t taddr, const Accumulators<PAIR> acc, uint32_t it, int more, int lane) {
+    return join_segments<BN, SPAN, PAIR>(taddr, acc, it, more, lane);
+}
+
+// The same where two accumulators take all of tensor memory: the sum waits in registers.  An f32 output
+// leaves from there, `cols` rows of it from `out` on, `step` apart, where the lane's channel is `live`, so that the next tile's segments go on meanwhile.  For a 16-bit one the sum is left in the last segment's
+// accumulator, which is not released.
+template <int BN, int SPAN, bool PAIR>
+__device__ __forceinline__ bool join_segments_wide(uint32_t taddr, const Accumulators<PAIR> acc, uint32_t it, int more, int lane,
+                                                bool f32, float *out, int64_t step, int cols, bool live) {
+    float sum[SPAN];
+    #pragma unroll
+    for (int c = 0; c < SPAN; ++c) sum[c] = 0.0f;
+    #pragma unroll 1
+    for (int s = 0;; ++s, ++it) {
+        if (!acc.wait(it, kLongSegment)) return false;
+        #pragma unroll
+        for (int c = 0; c < SPAN; c += 32) {
+            uint32_t r[32];
+            emmy::tmem_ld_32x32b_x32(taddr + (it & 1u) * BN + c, r);
+            emmy::tmem_ld_wait();
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
+        }
+        if (s == more) break;
+        acc.release(it, lane);
+    }
+    if (f32) {
+        acc.release(it, lane);
+        #pragma unroll
+        for (int c = 0; c < SPAN; ++c, out += step)
+            if (live && c < cols) *out = sum[c];
+        return true;
+    }
+    #pragma unroll
+    for (int c = 0; c < SPAN; c += 16) {
+        uint32_t r[16];
+        #pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(sum[c + j]);
+        emmy::tmem_st_32x32b_x16(taddr + (it & 1u) * BN + c, r);
+    }
+    emmy::tmem_st_wait();
+    return true;
+}
+
 // Send 16 columns' sums from `c` on, for one channel, to the CTAs that finish them: 16 / G columns to
 // each of G.  `own`: this rank's place in a CTA's exchange buffer, in bytes.
 template <int G>
@@ -527,8 +637,8 @@ struct TcConfig {
     static constexpr int kThreads = 64 + 32 * (kOut + kLoaders);
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kRed + kOutStage + 256;
     static constexpr int kPerSm = TMA && BN <= 32 ? 2 : 1;  // CTAs that share an SM
-    // two accumulators; store_tile reads 32 columns at a time, which may pass the second one's end
-    static constexpr uint32_t kTmemCols = BN >= 64 ? 4 * BN : 2 * BN;
+    // two accumulators and the columns of a third, in a power of two
+    static constexpr uint32_t kTmemCols = 4 * BN;
 };
 
 // One CTA on 128 channels x BN rows of output.  Warp 0 loads operand tiles by TMA (TMA false: the
@@ -548,7 +658,7 @@ struct TcConfig {
 // kernels that did so with more than 512 columns between them on one SM could block each other;
 // the CTAs here and those of the attention and GEMM families that take more than a few columns also
 // take more than half of an SM's shared memory, so no SM holds two of them.
-template <bool I8, int LAYOUT, int BN, bool TMA>
+template <bool I8, int LAYOUT, int BN, bool TMA, bool JOIN>
 __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, BN, TMA>::kPerSm)
     product_tc_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
                       const __grid_constant__ CUtensorMap tm_b) {
@@ -715,16 +825,28 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
             }
         } else if (warp == 1) {
             const Issue<I8, LAYOUT, false> issue(sA, sB, flags.bf16, BN);
+            const int segment = segment_blocks(p.out_type);
+            uint32_t d_tmem = tmem_base;
+            // waits for the accumulator of the tile's (segment's) sum
+            auto begin = [&] {
+                ok = __all_sync(0xffffffffu, emmy::mbar_wait(&tempty[it & 1u], (it >> 1 & 1u) ^ 1u, abort_flag,
+                                                             EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
+                emmy::tc_fence_after();
+                d_tmem = tmem_base + (it & 1u) * BN;
+            };
             for (int t = first; t < last && ok; t += step, ++it) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
-                const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
-                ok = __all_sync(0xffffffffu, emmy::mbar_wait(&tempty[acc], aphase ^ 1u, abort_flag,
-                                                             EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
-                if (!ok) break;
-                emmy::tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
                 const int blocks = uniform(w.kb1 - w.kb0), last_steps = uniform(last_block_steps(w, w.kb1, BK));
-                for (int i = 0; i < blocks; ++i) {
+                begin();
+                if (!ok) break;
+                for (int i = 0, from = 0; i < blocks; ++i) {
+                    if (JOIN && i == from + segment) {
+                        issue.commit(&tfull[it & 1u]);
+                        ++it;
+                        from = i;
+                        begin();
+                        if (!ok) break;
+                    }
                     ok = __all_sync(0xffffffffu, emmy::mbar_wait(&full[stage], phase, abort_flag,
                                                                  EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
                     if (!ok) break;
@@ -742,7 +864,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                         __syncwarp();
                     }
                     emmy::tc_fence_after();
-                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, i > 0, steps);
+                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, i > from, steps);
                     issue.commit(&empty[stage]);
                     if (++stage == STAGES) {
                         stage = 0;
@@ -750,23 +872,28 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                     }
                 }
                 if (!ok) break;
-                issue.commit(&tfull[acc]);
+                issue.commit(&tfull[it & 1u]);
             }
             __syncwarp();
         } else if (warp >= 2 && warp < 2 + Cfg::kOut) {
             const int q = warp & 3, part = (warp - 2) >> 2;
             constexpr int SPAN = BN / (Cfg::kOut / 4);
+            const Accumulators<false> acc{tfull, tempty, abort_flag};
             for (int t = first; t < last && ok; t += step, ++it) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
-                const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
                 const int64_t m = w.m0 + q * 32 + lane;
                 const Channel ch = channel<I8>(p, w, m);
                 RowScales<I8, (SPAN + 31) / 32> xs(p, w, part * SPAN, lane);
-                ok = __all_sync(0xffffffffu, emmy::mbar_wait(&tfull[acc], aphase, abort_flag,
-                                                             EMMY_STATUS_TIMEOUT_EPILOGUE, sum_wait_ns(w.kb1 - w.kb0)));
+                const uint32_t lanes = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+                const int more = JOIN ? more_segments(w.kb1 - w.kb0, segment_blocks(p.out_type)) : 0;
+                if constexpr (JOIN)
+                    ok = TMA ? join_segments<BN, SPAN, false>(lanes + part * SPAN, acc, it, more, lane)
+                             : join_segments_apart<BN, SPAN, false>(lanes + part * SPAN, acc, it, more, lane);
+                else
+                    ok = acc.wait(it, w.kb1 - w.kb0);
                 if (!ok) break;
-                emmy::tc_fence_after();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+                it += more;
+                const uint32_t taddr = lanes + (JOIN ? 2u : it & 1u) * BN;
                 const bool none = w.kb0 == w.kb1;  // nothing was accumulated
                 if (BN >= 64 && split == 1) {
                     store_tile<I8>(p, w, w.m0 + q * 32, taddr, none, part * SPAN, min((part + 1) * SPAN, w.cols), ch, xs,
@@ -798,9 +925,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
                         }
                     }
                 }
-                emmy::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) emmy::mbar_arrive(&tempty[acc]);
+                if (!JOIN) acc.release(it, lane);
             }
         }
         if (split > 1) {
@@ -921,13 +1046,14 @@ struct PairConfig {
     static constexpr uint32_t kStageB = BN / 2 * kBlockBytes;
     static constexpr uint32_t kStage = kStageA + kStageB;
     static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr uint32_t kTmemCols = 512;  // two accumulators, and the columns of a third of 128
     static constexpr int kOut = 8;  // warps that turn sums into output
     static constexpr int kThreads = 64 + 32 * kOut;
     static constexpr int kTailThreads = 32;  // dw: one more warp
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kOut * kStoreBytes + 512;
 };
 
-template <bool I8, int LAYOUT, int BN>
+template <bool I8, int LAYOUT, int BN, bool JOIN>
 __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? PairConfig<BN>::kTailThreads : 0), 1)
     product_pair_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
                         const __grid_constant__ CUtensorMap tm_b) {
@@ -965,7 +1091,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
         emmy::fence_barrier_init();
     }
     if (warp == 1) {
-        emmy::tmem_alloc_pair(tmem_holder, 2 * BN);
+        emmy::tmem_alloc_pair(tmem_holder, Cfg::kTmemCols);
         emmy::tmem_relinquish_pair();
     }
     if (warp == 0) {
@@ -1063,21 +1189,32 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
             const Issue<I8, LAYOUT, true> issue(sA, sB, flags.bf16, BN);
             uint32_t stage = 0, phase = 0, it = 0;
             bool ok = true;
+            const int segment = segment_blocks(p.out_type);
+            uint32_t d_tmem = tmem_base;
+            auto begin = [&] {
+                ok = __all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tempty[it & 1u], (it >> 1 & 1u) ^ 1u, abort_flag,
+                                                                     EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
+                emmy::tc_fence_after();
+                d_tmem = tmem_base + (it & 1u) * BN;
+            };
             for (int t = pair; t < total && ok; t += npairs, ++it) {
                 const Tile w = tile(t);
-                const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
-                ok = __all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tempty[acc], aphase ^ 1u, abort_flag,
-                                                                     EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
-                if (!ok) break;
-                emmy::tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
                 const int blocks = uniform(w.kb1), last_steps = uniform(last_block_steps(w, w.kb1, BK));
-                for (int i = 0; i < blocks; ++i) {
+                begin();
+                if (!ok) break;
+                for (int i = 0, from = 0; i < blocks; ++i) {
+                    if (JOIN && i == from + segment) {
+                        issue.commit(&tfull[it & 1u]);
+                        ++it;
+                        from = i;
+                        begin();
+                        if (!ok) break;
+                    }
                     ok = __all_sync(0xffffffffu, emmy::mbar_wait_cluster(&full[stage], phase, abort_flag,
                                                                          EMMY_STATUS_TIMEOUT_MMA, kWaitNs));
                     if (!ok) break;
                     emmy::tc_fence_after();
-                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, i > 0,
+                    issue.block(d_tmem, stage * kStageA, stage * Cfg::kStageB, i > from,
                                 LAYOUT == kMM && i == blocks - 1 ? last_steps : 4);
                     issue.commit(&empty[stage]);
                     if (++stage == STAGES) {
@@ -1086,7 +1223,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
                     }
                 }
                 if (!ok) break;
-                issue.commit(&tfull[acc]);
+                issue.commit(&tfull[it & 1u]);
             }
             // arrives on both CTAs once every pair MMA has finished
             issue.commit(drain);
@@ -1122,22 +1259,31 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
         // ---------------- output (both CTAs): own 128 channels of the tile
         const int q = warp & 3, part = (warp - 2) >> 2;
         constexpr int SPAN = BN / (Cfg::kOut / 4);
-        const uint32_t leader_tempty = emmy::mapa(&tempty[0], 0);
+        const Accumulators<true> acc{tfull, tempty, abort_flag};
         uint32_t it = 0;
         for (int t = pair; t < total; t += npairs, ++it) {
             const Tile w = tile(t);
-            const uint32_t acc = it & 1u, aphase = (it >> 1) & 1u;
             const Channel ch = channel<I8>(p, w, w.m0 + q * 32 + lane);
             const RowScales<I8, SPAN / 32> xs(p, w, part * SPAN, lane);
-            if (!__all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tfull[acc], aphase, abort_flag,
-                                                                 EMMY_STATUS_TIMEOUT_EPILOGUE, sum_wait_ns(w.kb1 - w.kb0))))
-                break;
-            emmy::tc_fence_after();
-            store_tile<I8>(p, w, w.m0 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, w.kb1 == 0,
-                           part * SPAN, min((part + 1) * SPAN, w.cols), ch, xs, sStore + (warp - 2) * kStoreBytes, lane);
-            emmy::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) emmy::mbar_arrive_cluster(leader_tempty + acc * 8u);
+            const uint32_t lanes = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+            const int more = JOIN ? more_segments(w.kb1, segment_blocks(p.out_type)) : 0, from = part * SPAN, m = w.m0 + q * 32;
+            constexpr bool WIDE = 3 * BN > 512;
+            const bool direct = WIDE && more && p.out_type == EMMY_F32;
+            bool ok;
+            if constexpr (JOIN && !WIDE)
+                ok = join_segments<BN, SPAN, true>(lanes + from, acc, it, more, lane);
+            else if (JOIN && more)
+                ok = join_segments_wide<BN, SPAN, true>(lanes + from, acc, it, more, lane, direct,
+                                                        static_cast<float *>(p.out) + out_index(p, w, m + lane, from), p.out_c,
+                                                        w.cols - from, m + lane < p.m);
+            else
+                ok = acc.wait(it, w.kb1);
+            if (!ok) break;
+            it += more;
+            if (direct) continue;
+            store_tile<I8>(p, w, m, lanes + (JOIN && !WIDE ? 2u : it & 1u) * BN, w.kb1 == 0, from, min(from + SPAN, w.cols), ch, xs,
+                           sStore + (warp - 2) * kStoreBytes, lane);
+            if (!JOIN || WIDE) acc.release(it, lane);
         }
     }
     emmy::tc_fence_before();
@@ -1153,7 +1299,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
     emmy::cluster_sync();  // no CTA leaves while its peer may still signal or read it
     if (warp == 1) {
         emmy::tc_fence_after();
-        emmy::tmem_dealloc_pair(tmem_base, 2 * BN);
+        emmy::tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
     }
 }
 

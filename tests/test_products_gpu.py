@@ -878,3 +878,80 @@ def test_a_launch_of_more_than_two_seconds():
             assert torch.equal(dw[i, a:a + 64, b:b + 64], want.float().to(BF16)), (i, a, b)
     del x, dw
     torch.cuda.empty_cache()
+
+
+def _positive(g, *shape, dtype=BF16, scale=1.0):
+    return (torch.rand(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def _product64(a, b):
+    """a.T @ b in 64 bits, some rows at a time."""
+    out = torch.zeros(a.shape[1], b.shape[1], dtype=torch.float64, device="cuda")
+    for i in range(0, a.shape[0], 16384):
+        out += a[i:i + 16384].double().t() @ b[i:i + 16384].double()
+    return out
+
+
+def _assert_long_sum(got, want, terms):
+    """A sum of ``terms`` products of one sign.  It is joined from parts of 1024 terms (f32 outputs) or 8192, which
+    lose at most a step (2^-23) of the sum for each term, in additions that lose at most half a step each;
+    then it is rounded to the output's type."""
+    part = 1024 if got.dtype == F32 else 8192
+    tol = (part + 2 + terms / part / 2) * 2.0 ** -23 * want + _half_step(got.dtype, want) * 1.01
+    bad = (got.double() - want).abs() > tol
+    assert not bad.any(), (int(bad.sum()), ((got.double() - want) / want).abs().max().item())
+
+
+# rows, n, k, kernel; the sums are n * k wide and as long as the rows
+LONG_DW = [(262144, 256, 256, (False, 128, 8)), (262144, 256, 255, (False, 128, 8)), (65536, 1024, 1280, (True, 128, 1)),
+           (65536, 1032, 2048, (True, 256, 1)), (262144, 1024, 1280, (True, 128, 1)), (65537, 1500, 1001, (False, 128, 1))]
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(BF16, F32), (F16, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("rows,n,k,kernel", LONG_DW)
+def test_long_sums_of_dw_keep_their_precision(rows, n, k, kernel, dtype, out_dtype):
+    g = _gen(rows + k)
+    assert products.variant(rows, 1, n, k, dw=True, aligned=n % 8 == 0 and k % 8 == 0) == kernel
+    dy, x = _positive(g, rows, n, dtype=dtype, scale=0.25), _positive(g, rows, k, dtype=dtype, scale=0.25)
+    dw = torch.empty(1, n, k, dtype=out_dtype, device="cuda")
+    products.grouped_matmul_dw(dy, x, _offsets([rows]), dw, stream=_stream())
+    _assert_long_sum(dw[0], _product64(dy, x), rows)
+
+
+# rows, n, kernel of sums of 32768 terms, or 32769
+LONG_FORWARD = [(300, 2048, 0, (False, 64, 1)), (2048, 2048, 0, (True, 256, 1)),
+                (12, 20000, 0, (False, 16, 1)), (24, 20000, 0, (False, 32, 1)), (100, 20000, 0, (True, 128, 1)),
+                (60, 20000, 0, (False, 128, 1)), (20, 300, 0, (False, 32, 8)), (100, 300, 0, (False, 64, 8)),
+                (30, 5000, 1, (False, 32, 2)), (100, 9000, 1, (False, 64, 1)), (1700, 1100, 1, (False, 128, 1))]
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(BF16, F32), (F16, F16)])
+@pytest.mark.parametrize("other_axis", [False, True])
+@pytest.mark.parametrize("rows,n,odd,kernel", LONG_FORWARD)
+def test_long_sums_keep_their_precision(rows, n, odd, kernel, other_axis, dtype, out_dtype):
+    g, k = _gen(rows + n), 32768 + odd
+    assert products.variant(rows, 1, n, k, aligned=not odd) == kernel
+    x = _positive(g, rows, k, dtype=dtype, scale=0.25)
+    w = _positive(g, 1, k, n, dtype=dtype, scale=0.25).transpose(1, 2) if other_axis else _positive(g, 1, n, k, dtype=dtype, scale=0.25)
+    out = torch.empty(rows, n, dtype=out_dtype, device="cuda")
+    products.grouped_matmul(x, w, _offsets([rows]), out, stream=_stream())
+    _assert_long_sum(out, _product64(x.t(), w[0].t()), k)
+
+
+def test_segments_of_many_groups():
+    """Sums of one segment, of several and of none follow one another on the same accumulators: exact integers."""
+    g = _gen(61)
+    counts, n, k = [512, 513, 0, 1023, 1024, 1025, 5, 4096, 4097, 2047, 0, 64], 776, 1032
+    rows, e, off = sum(counts), len(counts), _offsets(counts)
+    dy, x, w = _ints(g, rows, n), _ints(g, rows, k), _ints(g, e, n, k)
+    assert products.variant(rows, e, n, k, dw=True)[0] and products.variant(rows, e, n, k)[0]
+    dw, out, dx = torch.empty(e, n, k, device="cuda"), torch.empty(rows, n, device="cuda"), torch.empty(rows, k, device="cuda")
+    products.grouped_matmul_dw(dy, x, off, dw, stream=_stream())
+    products.grouped_matmul(x, w, off, out, stream=_stream())
+    products.grouped_matmul(dy, w.transpose(1, 2), off, dx, stream=_stream())
+    at = 0
+    for i, c in enumerate(counts):
+        D, X, W = dy[at:at + c].double(), x[at:at + c].double(), w[i].double()
+        assert torch.equal(dw[i].double(), D.t() @ X), c
+        assert torch.equal(out[at:at + c].double(), X @ W.t()) and torch.equal(dx[at:at + c].double(), D @ W), c
+        at += c
