@@ -153,19 +153,29 @@ def _inputs(case: dict, seed: int) -> dict:
 
 def prepare(case: dict, seed: int) -> dict:
     s = _inputs(case, seed)
-    # a decode loop works on the same buffers step after step, so it binds its calls once
     if own and case["tokens"] <= 64 and case["op"] != "backward":
-        from emmy_ptx_compiler_b200 import products
-
-        stream = torch.cuda.current_stream().cuda_stream
-        if case["op"] == "grouped":
-            s["calls"] = [products.bind_grouped_matmul(s["x"], s["w"], s["offsets"], s["out"], stream=stream)]
-        else:
-            s["calls"] = [products.bind_int8_matmul(s["xq"], s["xs"], s["wq"], s["ws"], s["out"],
-                                                    offsets=_groups(s), bias=s["bias"], stream=stream)]
-            if case["op"] == "linear8":
-                s["calls"].insert(0, products.bind_quantize_rows(s["x"], s["xq"], s["xs"], stream=stream))
+        _bind(s, _current_stream(s))
     return s
+
+
+def _current_stream(s: dict) -> int:
+    # what torch.cuda.current_stream().cuda_stream holds, without the 2 us of making its objects
+    return torch._C._cuda_getCurrentRawStream(s["out"].device.index)
+
+
+def _bind(s: dict, stream: int) -> None:
+    """The calls of a decode loop, which works on the same buffers step after step and so binds them once;
+    a bound call stays with its stream."""
+    from emmy_ptx_compiler_b200 import products
+
+    s["stream"] = stream
+    if s["case"]["op"] == "grouped":
+        s["calls"] = [products.bind_grouped_matmul(s["x"], s["w"], s["offsets"], s["out"], stream=stream)]
+        return
+    s["calls"] = [products.bind_int8_matmul(s["xq"], s["xs"], s["wq"], s["ws"], s["out"], offsets=_groups(s),
+                                            bias=s["bias"], stream=stream)]
+    if s["case"]["op"] == "linear8":
+        s["calls"].insert(0, products.bind_quantize_rows(s["x"], s["xq"], s["xs"], stream=stream))
 
 
 def _groups(s: dict):
@@ -177,6 +187,8 @@ def _run_own(s: dict):
 
     op = s["case"]["op"]
     if "calls" in s:
+        if s["stream"] != _current_stream(s):
+            _bind(s, _current_stream(s))
         for call in s["calls"]:
             call()
         return s["out"]
