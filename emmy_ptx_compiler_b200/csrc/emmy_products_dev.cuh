@@ -97,14 +97,4 @@ __device__ __forceinline__ void store_out(void *out, int type, int64_t i, float 
     }
 }
 
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(float v) { return v; }
-
-template <typename Acc, typename T>
-__device__ __forceinline__ Acc load_as(T v) {
-    if constexpr (sizeof(T) == 1) return v;
-    else return to_float(v);
-}
-
 }  // namespace
