@@ -365,7 +365,11 @@ int launch_single(const Launch &l) {
 template <bool I8, int LAYOUT, int BN, bool JOIN>
 int launch_pair(const Launch &l) {
     using Cfg = PairConfig<BN>;
-    static std::atomic<uint64_t> ready{0};
+    static std::atomic<uint64_t> ready{0}, ready_direct{0};
+    if constexpr (JOIN && BN == 256)
+        if (l.p.out_type == EMMY_F32)
+            return launch_clusters(l, product_pair_kernel<I8, LAYOUT, BN, JOIN, true>, ready_direct,
+                                   Cfg::kThreads + (LAYOUT == kMM ? Cfg::kTailThreads : 0), Cfg::kSmem);
     return launch_clusters(l, product_pair_kernel<I8, LAYOUT, BN, JOIN>, ready,
                            Cfg::kThreads + (LAYOUT == kMM ? Cfg::kTailThreads : 0), Cfg::kSmem);
 }

@@ -1,7 +1,7 @@
 // Products on the 5th-generation tensor cores: out(c, m) = sum_k A(m, k) B(c, k).
 //
 // The output's contiguous axis m (the channels) lies on the 128 lanes of tensor memory and the
-// output's rows c (the tokens of a group) on the N columns of the instruction, 16 to 128 of them.
+// output's rows c (the tokens of a group) on the N columns of the instruction, 16 to 256 of them.
 // So a group of a few tokens costs a few columns, not a padded tile of 128 rows, and a warp's
 // 32 lanes store 32 neighbouring channels of one output row.
 #pragma once
@@ -498,14 +498,19 @@ __device__ __forceinline__ void store_tile(const Product &p, const Tile &w, int 
 // Tensor cores cut off what lies below the last bit of a running sum, so a long sum of one sign would
 // lose up to half a step for each MMA (262144 rows of positive values: 1.5e-3 of their sum).  So sums of
 // 16-bit products are joined from segments, added in f32 to nearest by the warps that turn sums into
-// output: 1024 terms for an f32 output (1e-6 off for values of either sign, 1.7e-6 for values of one), 8192
-// where rounding to 16 bits follows (3e-5 of a sum of one sign; half a step is 4.9e-4 or 3.9e-3).
-// Kernels with JOIN do so, at 0 to 4 % more time (4 experts of 16384 rows, dw [2048, 2048]: 391 against
-// 385 us to bf16, 398 against 388 to f32); where no sum of a launch can be that long the others run.
-constexpr int kShortSegment = 16, kLongSegment = 128;  // blocks
+// output: up to 768 terms for an f32 output (0.7e-6 off for bf16 and 1.0e-6 for f16 values of either sign, 1.3e-6 and
+// 4.4e-6 for values of one), up to 8192 where rounding to 16 bits follows (5e-5 of a sum of one sign; half a
+// step is 4.9e-4 or 3.9e-3).  Kernels with JOIN do so, at 0 to 6 % more time (dw of 16384 rows each of 4
+// experts [2048, 2048]: 383 against 377 us to bf16, 386 against 381 to f32; 7108 rows, 24 experts [1416, 1000] to
+// f32: 44 against 41 us); where no sum of a launch can be that long the others run.
+constexpr int kShortSegment = 12, kLongSegment = 128;  // blocks
 __host__ __device__ constexpr int segment_blocks(int out_type) { return out_type == EMMY_F32 ? kShortSegment : kLongSegment; }
-// Segments of a sum after the first.
+// Segments of a sum after the first, and the blocks of each: as equal as they can be.
 __device__ __forceinline__ int more_segments(int blocks, int segment) { return blocks > segment ? (blocks - 1) / segment : 0; }
+__device__ __forceinline__ int equal_segment(int blocks, int segment) {
+    const int n = more_segments(blocks, segment) + 1;
+    return (blocks + n - 1) / n;
+}
 
 // The barriers of a tile's accumulators: segment `it` of a CTA's tiles arrives in accumulator `it` & 1.
 template <bool PAIR>
@@ -564,42 +569,42 @@ __device__ __noinline__ bool join_segments_apart(uint32_t taddr, const Accumulat
     return join_segments<BN, SPAN, PAIR>(taddr, acc, it, more, lane);
 }
 
-// The same where two accumulators take all of tensor memory: the sum waits in registers.  An f32 output
-// leaves from there, `cols` rows of it from `out` on, `step` apart, where the lane's channel is `live`, so that the next tile's segments go on meanwhile.  For a 16-bit one the sum is left in the last segment's
-// accumulator, which is not released.
-template <int BN, int SPAN, bool PAIR>
-__device__ __forceinline__ bool join_segments_wide(uint32_t taddr, const Accumulators<PAIR> acc, uint32_t it, int more, int lane,
-                                                bool f32, float *out, int64_t step, int cols, bool live) {
-    float sum[SPAN];
+// The same where two accumulators take all of tensor memory: the sum waits in registers.  The last segment's
+// accumulator is not released.  STEP: columns of a read (the compiler keeps all in registers at 16 where the sum
+// is stored from there, and at 32 where it goes back).
+template <int BN, int SPAN, int STEP, bool PAIR>
+__device__ __forceinline__ bool sum_segments(float (&sum)[SPAN], uint32_t taddr, const Accumulators<PAIR> &acc, uint32_t it, int more,
+                                             int lane) {
     #pragma unroll
     for (int c = 0; c < SPAN; ++c) sum[c] = 0.0f;
     #pragma unroll 1
     for (int s = 0;; ++s, ++it) {
         if (!acc.wait(it, kLongSegment)) return false;
         #pragma unroll
-        for (int c = 0; c < SPAN; c += 32) {
-            uint32_t r[32];
-            emmy::tmem_ld_32x32b_x32(taddr + (it & 1u) * BN + c, r);
+        for (int c = 0; c < SPAN; c += STEP) {
+            uint32_t r[STEP];
+            if constexpr (STEP == 32) emmy::tmem_ld_32x32b_x32(taddr + (it & 1u) * BN + c, r);
+            else emmy::tmem_ld_32x32b_x16(taddr + (it & 1u) * BN + c, r);
             emmy::tmem_ld_wait();
             #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < STEP; ++j) sum[c + j] += __uint_as_float(r[j]);
         }
-        if (s == more) break;
+        if (s == more) return true;
         acc.release(it, lane);
     }
-    if (f32) {
-        acc.release(it, lane);
-        #pragma unroll
-        for (int c = 0; c < SPAN; ++c, out += step)
-            if (live && c < cols) *out = sum[c];
-        return true;
-    }
+}
+
+// And put back into the last segment's accumulator.
+template <int BN, int SPAN, bool PAIR>
+__device__ __forceinline__ bool join_segments_wide(uint32_t taddr, const Accumulators<PAIR> &acc, uint32_t it, int more, int lane) {
+    float sum[SPAN];
+    if (!sum_segments<BN, SPAN, 32, PAIR>(sum, taddr, acc, it, more, lane)) return false;
     #pragma unroll
     for (int c = 0; c < SPAN; c += 16) {
         uint32_t r[16];
         #pragma unroll
         for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(sum[c + j]);
-        emmy::tmem_st_32x32b_x16(taddr + (it & 1u) * BN + c, r);
+        emmy::tmem_st_32x32b_x16(taddr + ((it + more) & 1u) * BN + c, r);
     }
     emmy::tmem_st_wait();
     return true;
@@ -655,9 +660,10 @@ struct TcConfig {
 // depends on no timing.
 //
 // Tensor memory is held from start to end, and the CTAs of a cluster wait for each other.  Two
-// kernels that did so with more than 512 columns between them on one SM could block each other;
-// the CTAs here and those of the attention and GEMM families that take more than a few columns also
-// take more than half of an SM's shared memory, so no SM holds two of them.
+// kernels that did so with more than 512 columns between them on one SM could block each other.  Shared
+// memory rules that out: a CTA with tiles of 16 or 32 rows (64 or 128 columns, up to 108 KB) leaves room for one
+// more of them or for one CTA of the attention family with at most 256 columns, and every CTA with
+// wider tiles, of the GEMM family or of the attention family with 512 columns takes 129 KB or more.
 template <bool I8, int LAYOUT, int BN, bool TMA, bool JOIN>
 __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, BN, TMA>::kPerSm)
     product_tc_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
@@ -825,7 +831,6 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
             }
         } else if (warp == 1) {
             const Issue<I8, LAYOUT, false> issue(sA, sB, flags.bf16, BN);
-            const int segment = segment_blocks(p.out_type);
             uint32_t d_tmem = tmem_base;
             // waits for the accumulator of the tile's (segment's) sum
             auto begin = [&] {
@@ -837,6 +842,7 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
             for (int t = first; t < last && ok; t += step, ++it) {
                 const Tile w = tile_at(p, g, t, mt, e, kTileM, BN, BK, rank, split);
                 const int blocks = uniform(w.kb1 - w.kb0), last_steps = uniform(last_block_steps(w, w.kb1, BK));
+                const int segment = JOIN ? uniform(equal_segment(blocks, segment_blocks(p.out_type))) : 0;
                 begin();
                 if (!ok) break;
                 for (int i = 0, from = 0; i < blocks; ++i) {
@@ -1053,7 +1059,8 @@ struct PairConfig {
     static constexpr uint32_t kSmem = 1024 + kStages * kStage + kOut * kStoreBytes + 512;
 };
 
-template <bool I8, int LAYOUT, int BN, bool JOIN>
+// DIRECT: f32 outputs of kernels with JOIN whose sums wait in registers.
+template <bool I8, int LAYOUT, int BN, bool JOIN, bool DIRECT = false>
 __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? PairConfig<BN>::kTailThreads : 0), 1)
     product_pair_kernel(const Product p, const Flags flags, const __grid_constant__ CUtensorMap tm_a,
                         const __grid_constant__ CUtensorMap tm_b) {
@@ -1189,7 +1196,6 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
             const Issue<I8, LAYOUT, true> issue(sA, sB, flags.bf16, BN);
             uint32_t stage = 0, phase = 0, it = 0;
             bool ok = true;
-            const int segment = segment_blocks(p.out_type);
             uint32_t d_tmem = tmem_base;
             auto begin = [&] {
                 ok = __all_sync(0xffffffffu, emmy::mbar_wait_cluster(&tempty[it & 1u], (it >> 1 & 1u) ^ 1u, abort_flag,
@@ -1200,6 +1206,7 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
             for (int t = pair; t < total && ok; t += npairs, ++it) {
                 const Tile w = tile(t);
                 const int blocks = uniform(w.kb1), last_steps = uniform(last_block_steps(w, w.kb1, BK));
+                const int segment = JOIN ? uniform(equal_segment(blocks, segment_blocks(p.out_type))) : 0;
                 begin();
                 if (!ok) break;
                 for (int i = 0, from = 0; i < blocks; ++i) {
@@ -1267,23 +1274,31 @@ __global__ void __launch_bounds__(PairConfig<BN>::kThreads + (LAYOUT == kMM ? Pa
             const RowScales<I8, SPAN / 32> xs(p, w, part * SPAN, lane);
             const uint32_t lanes = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
             const int more = JOIN ? more_segments(w.kb1, segment_blocks(p.out_type)) : 0, from = part * SPAN, m = w.m0 + q * 32;
-            constexpr bool WIDE = 3 * BN > 512;
-            const bool direct = WIDE && more && p.out_type == EMMY_F32;
-            bool ok;
-            if constexpr (JOIN && !WIDE)
-                ok = join_segments<BN, SPAN, true>(lanes + from, acc, it, more, lane);
-            else if (JOIN && more)
-                ok = join_segments_wide<BN, SPAN, true>(lanes + from, acc, it, more, lane, direct,
-                                                        static_cast<float *>(p.out) + out_index(p, w, m + lane, from), p.out_c,
-                                                        w.cols - from, m + lane < p.m);
-            else
-                ok = acc.wait(it, w.kb1);
-            if (!ok) break;
-            it += more;
-            if (direct) continue;
-            store_tile<I8>(p, w, m, lanes + (JOIN && !WIDE ? 2u : it & 1u) * BN, w.kb1 == 0, from, min(from + SPAN, w.cols), ch, xs,
-                           sStore + (warp - 2) * kStoreBytes, lane);
-            if (!JOIN || WIDE) acc.release(it, lane);
+            if constexpr (DIRECT) {
+                // f32 sums leave from registers while the next tile's segments go on
+                float sum[SPAN], *out = static_cast<float *>(p.out) + out_index(p, w, m + lane, from);
+                const int cols = m + lane < p.m ? w.cols - from : 0;
+                if (!sum_segments<BN, SPAN, 16, true>(sum, lanes + from, acc, it, more, lane)) break;
+                it += more;
+                acc.release(it, lane);
+                #pragma unroll
+                for (int c = 0; c < SPAN; ++c, out += p.out_c)
+                    if (c < cols) *out = w.kb1 == 0 ? 0.0f : sum[c];
+            } else {
+                constexpr bool WIDE = 3 * BN > 512;
+                bool ok;
+                if constexpr (JOIN && !WIDE)
+                    ok = join_segments<BN, SPAN, true>(lanes + from, acc, it, more, lane);
+                else if (JOIN && more)
+                    ok = join_segments_wide<BN, SPAN, true>(lanes + from, acc, it, more, lane);
+                else
+                    ok = acc.wait(it, w.kb1);
+                if (!ok) break;
+                it += more;
+                store_tile<I8>(p, w, m, lanes + (JOIN && !WIDE ? 2u : it & 1u) * BN, w.kb1 == 0, from, min(from + SPAN, w.cols), ch,
+                               xs, sStore + (warp - 2) * kStoreBytes, lane);
+                if (!JOIN || WIDE) acc.release(it, lane);
+            }
         }
     }
     emmy::tc_fence_before();

@@ -147,8 +147,8 @@ def grouped_matmul(x, w, offsets, out, stream: int = 0) -> None:
 
     ``x`` [rows, k], ``w`` [experts, n, k] of the same type (bfloat16 or float16) with either of its
     last two axes contiguous, ``out`` [rows, n] of that type or float32.  Sums are held in f32 and
-    rounded once.  Tensor cores truncate where they add: a float32 output is off by about 1e-6 of its
-    size, 2e-6 where all products have one sign and towards zero, however many terms it has."""
+    rounded once.  Tensor cores truncate where they add: a float32 output is off by up to 1e-6 of its
+    size, or 5e-6 and towards zero where all products have one sign, however many terms it has."""
     bind_grouped_matmul(x, w, offsets, out, stream)()
 
 

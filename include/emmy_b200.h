@@ -214,10 +214,10 @@ int emmy_sum_f32_noalloc(int dev, const float *x, uint64_t n, float *out, uint64
  *
  * Types: EMMY_BF16 or EMMY_F16 operands with f32 accumulation, outputs of the
  * operands' type or EMMY_F32; 8-bit integers accumulate in s32, which is exact for
- * k <= EMMY_PRODUCTS_MAX_K8.  Tensor cores truncate where they add: a f32 sum
- * of any length is off by about 1e-6 of its size for products of either sign
- * and 2e-6 for products of one sign, always towards zero.  Before a 16-bit
- * output is rounded it is off by up to 3e-5.
+ * k <= EMMY_PRODUCTS_MAX_K8.  Tensor cores truncate where they add: an f32 sum
+ * of any length is off by up to 1e-6 of its size where products have either
+ * sign, and by up to 5e-6, towards zero, where they have one.  Before a 16-bit
+ * output is rounded it is off by up to 5e-5.
  *
  *   emmy_grouped_matmul     out[r, :] = sum_k x[r, k] * w[e, :, k] for the rows r
  *                           of expert e.  One of w's strides over n and k is 1.

@@ -861,11 +861,11 @@ def test_split_sums_of_dw_are_exact(rows, n, k, split):
 
 def test_a_launch_of_more_than_two_seconds():
     """The blocks that end inside come last, in an expert of their own: what waits for them waits for
-    the whole launch, 4e15 operations (2.4 s at 1.65 PFLOP/s), and this is no failure."""
-    n, rows, last = 73728, 368_000, 33
+    the whole launch, 2.8e15 operations (2.9 s), and this is no failure."""
+    n, rows, last = 73728, 256_000, 33
     torch.cuda.empty_cache()
-    if torch.cuda.mem_get_info()[0] < 85 << 30:
-        pytest.skip("needs 76 GB of device memory")
+    if torch.cuda.mem_get_info()[0] < 70 << 30:
+        pytest.skip("needs 60 GB of device memory")
     assert rows % 64 == 0 and products.variant(rows + last, 2, n, n, dw=True) == (True, 256, 1)
     x = torch.empty(rows + last, n, dtype=BF16, device="cuda").random_(-3, 4, generator=_gen(51))
     dw = torch.empty(2, n, n, dtype=BF16, device="cuda")
@@ -893,10 +893,10 @@ def _product64(a, b):
 
 
 def _assert_long_sum(got, want, terms):
-    """A sum of ``terms`` products of one sign.  It is joined from parts of 1024 terms (f32 outputs) or 8192, which
+    """A sum of ``terms`` products of one sign.  It is joined from parts of 768 terms (f32 outputs) or 8192, which
     lose at most a step (2^-23) of the sum for each term, in additions that lose at most half a step each;
     then it is rounded to the output's type."""
-    part = 1024 if got.dtype == F32 else 8192
+    part = 768 if got.dtype == F32 else 8192
     tol = (part + 2 + terms / part / 2) * 2.0 ** -23 * want + _half_step(got.dtype, want) * 1.01
     bad = (got.double() - want).abs() > tol
     assert not bad.any(), (int(bad.sum()), ((got.double() - want) / want).abs().max().item())
@@ -941,7 +941,7 @@ def test_long_sums_keep_their_precision(rows, n, odd, kernel, other_axis, dtype,
 def test_segments_of_many_groups():
     """Sums of one segment, of several and of none follow one another on the same accumulators: exact integers."""
     g = _gen(61)
-    counts, n, k = [512, 513, 0, 1023, 1024, 1025, 5, 4096, 4097, 2047, 0, 64], 776, 1032
+    counts, n, k = [768, 769, 0, 1023, 1536, 1537, 5, 4096, 4097, 9000, 0, 64], 776, 1032
     rows, e, off = sum(counts), len(counts), _offsets(counts)
     dy, x, w = _ints(g, rows, n), _ints(g, rows, k), _ints(g, e, n, k)
     assert products.variant(rows, e, n, k, dw=True)[0] and products.variant(rows, e, n, k)[0]
