@@ -56,9 +56,9 @@ namespace {
 //   it is a multiple of half a step of s and at most about s / 2, so the FMA that computes it is
 //   exact, and comparing it with s / 2 settles the side and the ties.
 //
-// 16381 x 8192 f32 rows take 106 us (6.3 TB/s), bf16 rows 75 to 82 us (4.9 to 5.4 TB/s), which issue
-// instructions in 7 of 10 cycles: the more of their quotients lie near a half, the longer.  One row
-// takes 2 us.
+// 16381 x 8192 f32 rows take 107 us (6.2 TB/s), 16-bit rows 72 to 82 us (4.9 to 5.6 TB/s), which issue
+// instructions in 7 of 10 cycles: the more of their quotients lie near a half, the longer (rows of small
+// integers, where most packs hold one, 100 us).  One row takes 2 us.
 
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
 constexpr float kNearHalf = 0.49999f;  // below: off by less than 127.5 * 2^-24 = 7.6e-6

@@ -1040,8 +1040,8 @@ __global__ void __launch_bounds__(TcConfig<I8, BN, TMA>::kThreads, TcConfig<I8, 
 // A pair moves 64 bytes into shared memory per SM and clock of MMA (BN = 256), half of what a
 // single CTA's 128 x 128 tile needs.
 //
-// Bound by the tensor cores where sums are long: 16384 rows, 4 experts [4096, 4096], take 345 us (1.59
-// PFLOP/s bf16), int8 8192^3 takes 318 us (3.46 POP/s).  Sums of a few blocks are bound by the way
+// Bound by the tensor cores where sums are long: 16384 rows, 4 experts [4096, 4096], take 347 us (1.58
+// PFLOP/s bf16), int8 8192^3 takes 326 us (3.38 POP/s).  Sums of a few blocks are bound by the way
 // out (a 32 x 32 piece of a tile takes its warp 800 cycles): 8192 rows, 32 experts, dx [1024, 512] 20 us.
 // Measured on the way: 6 stages against 4, 352 against 382 us for the first of these; MMAs issued
 // from a branch of one lane, with their operands moved to uniform registers one by one, 590 cycles a
