@@ -182,3 +182,15 @@ def test_the_gpu_tests_reach_every_kernel():
     every |= {(True, (True, w)) for w in (128, 256)}
     assert forward == every and rows_gradient == every and int8 == every
     assert dw == {(True, (False, 128)), (False, (False, 128)), (True, (True, 128)), (True, (True, 256))}
+
+
+def test_the_gpu_tests_reach_every_kernel_with_long_sums():
+    import test_products_gpu as gpu
+
+    every = {(0, (False, w)) for w in (16, 32, 64, 128)} | {(1, (False, w)) for w in (32, 64, 128)}
+    every |= {(0, (True, w)) for w in (128, 256)}
+    assert {(odd, kernel[:2]) for _, _, odd, kernel in gpu.LONG_FORWARD} == every
+    for rows, n, odd, kernel in gpu.LONG_FORWARD:
+        assert products.variant(rows, 1, n, 32768 + odd, aligned=not odd) == kernel
+    reached = {(n % 8 == 0 and k % 8 == 0, kernel[:2]) for _, n, k, kernel in gpu.LONG_DW}
+    assert reached == {(True, (False, 128)), (False, (False, 128)), (True, (True, 128)), (True, (True, 256))}

@@ -955,3 +955,27 @@ def test_segments_of_many_groups():
         assert torch.equal(dw[i].double(), D.t() @ X), c
         assert torch.equal(out[at:at + c].double(), X @ W.t()) and torch.equal(dx[at:at + c].double(), D @ W), c
         at += c
+
+
+def test_kernels_of_every_width_at_once():
+    """Divided and joined sums of all tile widths on streams of their own: what they hold of an SM leaves
+    room for the others, and none waits for good."""
+    g = _gen(71)
+    calls, checks = [], []
+    for rows, n in ((9, 136), (20, 136), (9, 4112), (20, 4112), (40, 136), (100, 2080), (600, 2600), (2048, 2048)):
+        k, s = 8192, torch.cuda.Stream()
+        x, w, off, out = _ints(g, rows, k), _ints(g, 1, n, k), _offsets([rows]), torch.empty(rows, n, device="cuda")
+        calls.append(products.bind_grouped_matmul(x, w, off, out, stream=s.cuda_stream))
+        checks.append((out, x.double() @ w[0].double().t()))
+    for rows, n, k in ((9000, 72, 72), (5000, 1032, 1032), (3000, 777, 129)):
+        s = torch.cuda.Stream()
+        dy, x, off, dw = _ints(g, rows, n), _ints(g, rows, k), _offsets([rows]), torch.empty(1, n, k, device="cuda")
+        calls.append(products.bind_grouped_matmul_dw(dy, x, off, dw, stream=s.cuda_stream))
+        checks.append((dw[0], dy.double().t() @ x.double()))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for call in calls:
+            call()
+    torch.cuda.synchronize()
+    for out, want in checks:
+        assert torch.equal(out.double(), want)
